@@ -325,6 +325,142 @@ int lkhip_attn_decode_noalloc(const float* q, const uint16_t* k_cache, const uin
 /* Greedy argmax (src/sampler.rs:67-75, first max wins) of n_rows rows of n. */
 int lkhip_argmax(const float* x, size_t n_rows, size_t n, uint32_t* out, void* stream);
 
+/* ---------------------------------------------------- paged KV cache */
+
+/* The kernel-level calls below keep and read a KV cache of pages: fixed runs
+ * of positions that sequences hold in any order and may share.  The reference
+ * has no such cache; its callers that need one are the server (several
+ * sequences, src/engine.rs:38-48) and speculative decoding
+ * (src/generate.rs:152-268).  As all kernel-level calls they take DEVICE
+ * pointers and a stream, allocate nothing and do not synchronise, so they can
+ * be captured into a graph; descriptors are read during the call only.
+ *
+ * What lies in device memory cannot be refused by the host: a slot at or above
+ * n_seq, a position behind the table and a page id at or above n_pages (as
+ * LKHIP_NO_PAGE) are looked at by the kernels, which skip such a sequence or
+ * row and treat such a page as a hole whose positions nobody sees. */
+#define LKHIP_NO_PAGE 0xFFFFFFFFu
+
+/* The pools.  Element d of row o (o < page_size) of page p, layer l and kv
+ * head h is at l * layer_stride + p * page_stride + h * head_stride +
+ * o * head_dim + d, counted in elements of kv_type (LKHIP_F16 or LKHIP_F32),
+ * in k and in v.  head_dim 64 or 128, page_size 16, 32, 64, 128 or 256; k, v
+ * 16-byte aligned; a stride whose count is above 1 is a multiple of 16 bytes
+ * and at least a page's rows of one head.  Every id below n_pages must name
+ * memory of the pools for every head and layer.  (A slot cache
+ * [slot][kv_head][max_seq][head_dim] is one with page_stride = page_size *
+ * head_dim, head_stride = max_seq * head_dim, page i of a slot being
+ * slot * n_kv_heads * (max_seq / page_size) + i, and n_pages one more than the
+ * last slot's last page.) */
+typedef struct lkhip_kv_pages {
+    void* k;
+    void* v;
+    uint32_t kv_type;
+    uint32_t head_dim;
+    uint32_t n_kv_heads;
+    uint32_t page_size;
+    uint32_t n_layers;
+    uint32_t reserved; /* 0 */
+    uint64_t n_pages;
+    uint64_t page_stride;
+    uint64_t head_stride;
+    uint64_t layer_stride;
+} lkhip_kv_pages;
+
+/* Which pages sequences hold, shared by all layers (device u32 arrays):
+ * table[n_seq][max_pages] ids, LKHIP_NO_PAGE behind a sequence's last page;
+ * len[n_seq] positions held; refs[n_pages] how many tables hold a page, 0 for
+ * a free one.  max_pages * page_size < 2^31.  lkhip_pages_fork / grow / trim
+ * keep the three together: start with refs and len 0 and every id
+ * LKHIP_NO_PAGE.  The other calls read table alone (len, refs may be NULL). */
+typedef struct lkhip_page_table {
+    uint32_t* table;
+    uint32_t* len;
+    uint32_t* refs;
+    uint32_t n_seq;
+    uint32_t max_pages;
+} lkhip_page_table;
+
+/* Sequence dst[i] becomes src[i]'s twin: it holds the same pages (refs + 1),
+ * nothing is copied.  ok[i] = 1, or 0 and nothing done where a slot does not
+ * exist, dst[i] holds something or was named before, or src[i] is a dst of
+ * the call.  n <= 1024. */
+int lkhip_pages_fork(const lkhip_kv_pages* pages, const lkhip_page_table* table, const uint32_t* src,
+                     const uint32_t* dst, size_t n, uint32_t* ok, void* stream);
+/* Makes room for add[i] more positions of sequence slots[i] (len += add) with
+ * the lowest free pages, in list order.  A last page that is not full and that
+ * another sequence holds too is first replaced by a copy of its rows, in all
+ * layers: copied[2 i], [2 i + 1] = the old and the new page, else
+ * LKHIP_NO_PAGE.  ok[i] = 1, or 0 and nothing done where the slot does not
+ * exist, was named before, the table is too short or the free pages end before
+ * this entry's last one (entries behind it that need any are refused with it).
+ * n <= 1024. */
+int lkhip_pages_grow(const lkhip_kv_pages* pages, const lkhip_page_table* table, const uint32_t* slots,
+                     const uint32_t* add, size_t n, uint32_t* ok, uint32_t* copied, void* stream);
+/* Sequence slots[i] keeps its first min(keep[i], len) positions and gives back
+ * the pages behind them (refs - 1; a page is free at 0); keep 0 frees it.  A
+ * slot named twice is taken at its first place.  n <= 1024. */
+int lkhip_pages_trim(const lkhip_kv_pages* pages, const lkhip_page_table* table, const uint32_t* slots,
+                     const uint32_t* keep, size_t n, void* stream);
+/* Row r of k and v (n_kv_heads * head_dim f32, ld floats apart, ld % 4 == 0,
+ * 16-byte aligned) becomes position pos[r] of sequence slots[r] in one layer,
+ * rounded to the cache's type (to nearest, as lokal's GPU cache,
+ * src/gpu/metal.rs:3234-3235).  Rows of a call must have different places. */
+int lkhip_pages_write(const lkhip_kv_pages* pages, const lkhip_page_table* table, uint32_t layer, const float* k,
+                      const float* v, size_t ld, const uint32_t* slots, const uint32_t* pos, size_t n_rows,
+                      void* stream);
+/* The rows at positions from[i] + path[i][j] of sequence slots[i] move to
+ * from[i] + j, j < n_path[i], in all layers: the accepted tokens of a draft
+ * close up behind their context.  path: [n][ld_path], strictly increasing (it
+ * ends at an entry that is not).  Rows in holes are left.  A slot named twice
+ * is taken at its first place.  n <= 1024. */
+int lkhip_pages_compact(const lkhip_kv_pages* pages, const lkhip_page_table* table, const uint32_t* slots,
+                        const uint32_t* from, const uint32_t* path, size_t ld_path, const uint32_t* n_path, size_t n,
+                        void* stream);
+/* Attention of drafted tokens (a tree of them, src/generate.rs:152-268 drafts
+ * a chain) over a cache that holds them behind their context.  q, out:
+ * [n][max_draft][n_heads * head_dim] f32.  Token t < n_draft[i] of sequence
+ * slots[i] (NULL: i) sees the positions 0..ctx_len[i]-1 and, at ctx_len[i] + j,
+ * the drafted tokens j < n_draft[i] whose bit is set: bit j % 32 of
+ * mask[i][t][j / 32], [n][max_draft][ceil(max_draft / 32)] words; mask NULL: j
+ * <= t.  Softmax of q.k / sqrt(head_dim) in f32; a row that sees nothing gives
+ * zeros; rows at and behind n_draft[i] are left as they were.  n_draft NULL: all have max_draft (<= 1024).
+ * n_heads: a multiple of the kv heads.  Positions that a row does not see do
+ * not reach it, whatever they hold; one that it sees with a K or V that is not
+ * finite makes it not finite.  Needs lkhip_tree_attn_workspace bytes (16-byte
+ * aligned, any content), in use until the call's work is done: two calls that
+ * can run at once need two. */
+int lkhip_tree_attn_workspace(const lkhip_kv_pages* pages, const lkhip_page_table* table, size_t n, size_t max_draft,
+                              size_t n_heads, size_t* bytes);
+int lkhip_tree_attn(const lkhip_kv_pages* pages, const lkhip_page_table* table, uint32_t layer, const float* q,
+                    const uint32_t* slots, const uint32_t* ctx_len, const uint32_t* n_draft, const uint32_t* mask,
+                    size_t n, size_t max_draft, size_t n_heads, void* ws, size_t ws_bytes, float* out, void* stream);
+/* The smallest and largest key of each dim over the live rows of the pages
+ * that hold positions from[i]..to[i]-1 of sequence slots[i] (NULL: i) in one
+ * layer; rows at and behind to[i] do not count, a NaN does.  bounds:
+ * [n_pages][n_kv_heads][2][head_dim] in the cache's type, one such array per
+ * layer; pages not touched keep theirs.  Entries of a call that share a page
+ * must agree on its live rows. */
+int lkhip_page_bounds(const lkhip_kv_pages* pages, const lkhip_page_table* table, uint32_t layer,
+                      const uint32_t* slots, const uint32_t* from, const uint32_t* to, size_t n, void* bounds,
+                      void* stream);
+/* Attention of one token per sequence over n_take of its pages, chosen per kv
+ * head: the first n_first, the last n_last, and of the others those whose
+ * bounds (lkhip_page_bounds) let a q.k be largest, i.e. by
+ * max over the kv head's query heads of sum_d max(q_d * min_d, q_d * max_d),
+ * taken in f64; a NaN counts as largest, equal ones go to the lowest page.
+ * n_first + n_last <= n_take.  taken: [n][n_kv_heads][n_take] page numbers
+ * within the sequence (not ids), ascending, LKHIP_NO_PAGE behind the last; a
+ * sequence of at most n_take pages is read whole.  q, out: [n][n_heads *
+ * head_dim] f32; ctx_len[i] positions are live, the token's own among them; 0:
+ * zeros.  The rest as lkhip_tree_attn. */
+int lkhip_sparse_attn_workspace(const lkhip_kv_pages* pages, const lkhip_page_table* table, size_t n, size_t n_heads,
+                                size_t n_take, size_t* bytes);
+int lkhip_sparse_attn(const lkhip_kv_pages* pages, const lkhip_page_table* table, uint32_t layer, const float* q,
+                      const uint32_t* slots, const uint32_t* ctx_len, const void* bounds, size_t n, size_t n_heads,
+                      size_t n_take, size_t n_first, size_t n_last, uint32_t* taken, void* ws, size_t ws_bytes,
+                      float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -56,10 +56,27 @@ class Profile(C.Structure):
         return {k: getattr(self, k) for k, _ in self._fields_}
 
 
+class KvPagesDesc(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("kv_type", C.c_uint32), ("head_dim", C.c_uint32),
+        ("n_kv_heads", C.c_uint32), ("page_size", C.c_uint32), ("n_layers", C.c_uint32), ("reserved", C.c_uint32),
+        ("n_pages", C.c_uint64), ("page_stride", C.c_uint64), ("head_stride", C.c_uint64), ("layer_stride", C.c_uint64),
+    ]
+
+
+class PageTableDesc(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p), ("len", C.c_void_p), ("refs", C.c_void_p), ("n_seq", C.c_uint32),
+        ("max_pages", C.c_uint32),
+    ]
+
+
 _P = C.c_void_p
 _F = C.POINTER(C.c_float)
 _U32 = C.POINTER(C.c_uint32)
 _U16 = C.POINTER(C.c_uint16)
+_Z = C.c_size_t
+_PAGED = [C.POINTER(KvPagesDesc), C.POINTER(PageTableDesc)]
 
 # name -> (restype, argtypes); mirrors include/lokal_hip.h one to one.
 SIGNATURES = {
@@ -127,6 +144,16 @@ SIGNATURES = {
     "lkhip_attn_decode_noalloc": (C.c_int, [_P, _P, _P, _P, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t,
                                             C.c_size_t, _P, _P]),
     "lkhip_argmax": (C.c_int, [_P, C.c_size_t, C.c_size_t, _P, _P]),
+    "lkhip_pages_fork": (C.c_int, _PAGED + [_P, _P, _Z, _P, _P]),
+    "lkhip_pages_grow": (C.c_int, _PAGED + [_P, _P, _Z, _P, _P, _P]),
+    "lkhip_pages_trim": (C.c_int, _PAGED + [_P, _P, _Z, _P]),
+    "lkhip_pages_write": (C.c_int, _PAGED + [C.c_uint32, _P, _P, _Z, _P, _P, _Z, _P]),
+    "lkhip_pages_compact": (C.c_int, _PAGED + [_P, _P, _P, _Z, _P, _Z, _P]),
+    "lkhip_tree_attn_workspace": (C.c_int, _PAGED + [_Z, _Z, _Z, C.POINTER(_Z)]),
+    "lkhip_tree_attn": (C.c_int, _PAGED + [C.c_uint32, _P, _P, _P, _P, _P, _Z, _Z, _Z, _P, _Z, _P, _P]),
+    "lkhip_page_bounds": (C.c_int, _PAGED + [C.c_uint32, _P, _P, _P, _Z, _P, _P]),
+    "lkhip_sparse_attn_workspace": (C.c_int, _PAGED + [_Z, _Z, _Z, C.POINTER(_Z)]),
+    "lkhip_sparse_attn": (C.c_int, _PAGED + [C.c_uint32, _P, _P, _P, _P, _Z, _Z, _Z, _Z, _Z, _P, _P, _Z, _P, _P]),
 }
 
 _lib = None

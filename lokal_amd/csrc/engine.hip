@@ -38,6 +38,11 @@ static int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+int lk_fail(int code, const char* why) {
+    g_err = why;
+    return code;
+}
+
 #define HIP_OR_FAIL(expr)                                                                                  \
     do {                                                                                                   \
         hipError_t _e = (expr);                                                                            \

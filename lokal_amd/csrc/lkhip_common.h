@@ -8,6 +8,9 @@
 
 #define LK_WAVE 64
 
+// Sets this thread's lkhip_last_error text and returns code (engine.hip).
+int lk_fail(int code, const char* why);
+
 // Weight types as stored on the device (GGUF ids; values unchanged, layout
 // repacked).  LK_Q8_SM is not a GGUF type: it is the device form of Q6_K and
 // Q5_K (see LkDevW).  Q4_0 and Q5_0 are stored as LK_Q8_0.

@@ -11,7 +11,10 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import check, lib
+from ._lib import LKHIP_F16, LKHIP_F32, KvPagesDesc, PageTableDesc, check, lib
+
+F16, F32 = LKHIP_F16, LKHIP_F32  # KV cache types
+NO_PAGE = 0xFFFFFFFF
 
 
 class DeviceArray:
@@ -147,6 +150,96 @@ def attn_decode_noalloc(q: DeviceArray, k: DeviceArray, v: DeviceArray, ctx_len:
 
 def argmax(x: DeviceArray, n_rows: int, n: int, out: DeviceArray, stream=None) -> None:
     check(lib().lkhip_argmax(x.ptr, n_rows, n, out.ptr, stream))
+
+
+# ------------------------------------------------------------ paged KV cache
+
+class KvPages:
+    """K and V pools of pages (lkhip_kv_pages); strides in elements, dense [layer][page][kv head][row][dim] if left out."""
+
+    def __init__(self, k: DeviceArray, v: DeviceArray, kv_type: int, n_layers: int, n_pages: int, n_kv_heads: int,
+                 page_size: int, head_dim: int, page_stride: int | None = None, head_stride: int | None = None,
+                 layer_stride: int | None = None):
+        head = page_size * head_dim if head_stride is None else head_stride
+        page = n_kv_heads * page_size * head_dim if page_stride is None else page_stride
+        layer = n_pages * n_kv_heads * page_size * head_dim if layer_stride is None else layer_stride
+        self.k, self.v = k, v
+        self.desc = KvPagesDesc(k.ptr, v.ptr, kv_type, head_dim, n_kv_heads, page_size, n_layers, 0, n_pages, page,
+                                head, layer)
+        self._ref = C.byref(self.desc)
+
+
+class PageTable:
+    """Page ids [n_seq][max_pages], lengths and reference counts (lkhip_page_table); the last two may be None where
+    pages_fork / pages_grow / pages_trim are not used."""
+
+    def __init__(self, table: DeviceArray, length: DeviceArray | None, refs: DeviceArray | None, n_seq: int,
+                 max_pages: int):
+        self.table, self.length, self.refs = table, length, refs
+        self.desc = PageTableDesc(table.ptr, _p(length), _p(refs), n_seq, max_pages)
+        self._ref = C.byref(self.desc)
+
+
+def pages_fork(pages: KvPages, table: PageTable, src: DeviceArray, dst: DeviceArray, n: int, ok: DeviceArray,
+               stream=None) -> None:
+    check(lib().lkhip_pages_fork(pages._ref, table._ref, src.ptr, dst.ptr, n, ok.ptr, stream))
+
+
+def pages_grow(pages: KvPages, table: PageTable, slots: DeviceArray, add: DeviceArray, n: int, ok: DeviceArray,
+               copied: DeviceArray, stream=None) -> None:
+    check(lib().lkhip_pages_grow(pages._ref, table._ref, slots.ptr, add.ptr, n, ok.ptr, copied.ptr, stream))
+
+
+def pages_trim(pages: KvPages, table: PageTable, slots: DeviceArray, keep: DeviceArray, n: int, stream=None) -> None:
+    check(lib().lkhip_pages_trim(pages._ref, table._ref, slots.ptr, keep.ptr, n, stream))
+
+
+def pages_write(pages: KvPages, table: PageTable, layer: int, k: DeviceArray, v: DeviceArray, slots: DeviceArray,
+                pos: DeviceArray, n_rows: int, ld: int | None = None, stream=None) -> None:
+    d = pages.desc
+    check(lib().lkhip_pages_write(pages._ref, table._ref, layer, k.ptr, v.ptr, ld or d.n_kv_heads * d.head_dim,
+                                  slots.ptr, pos.ptr, n_rows, stream))
+
+
+def pages_compact(pages: KvPages, table: PageTable, slots: DeviceArray, start: DeviceArray, path: DeviceArray,
+                  n_path: DeviceArray, n: int, ld_path: int, stream=None) -> None:
+    check(lib().lkhip_pages_compact(pages._ref, table._ref, slots.ptr, start.ptr, path.ptr, ld_path, n_path.ptr, n,
+                                    stream))
+
+
+def tree_attn_workspace(pages: KvPages, table: PageTable, n: int, max_draft: int, n_heads: int) -> int:
+    b = C.c_size_t()
+    check(lib().lkhip_tree_attn_workspace(pages._ref, table._ref, n, max_draft, n_heads, C.byref(b)))
+    return b.value
+
+
+def tree_attn(pages: KvPages, table: PageTable, layer: int, q: DeviceArray, ctx_len: DeviceArray,
+              n_draft: DeviceArray | None, mask: DeviceArray | None, n: int, max_draft: int, n_heads: int,
+              ws: DeviceArray | None, ws_bytes: int, out: DeviceArray, slots: DeviceArray | None = None,
+              stream=None) -> None:
+    """Drafted tokens over their contexts: out[i, t] for t < n_draft[i], seeing what mask's bits allow of the draft."""
+    check(lib().lkhip_tree_attn(pages._ref, table._ref, layer, q.ptr, _p(slots), ctx_len.ptr, _p(n_draft), _p(mask), n,
+                                max_draft, n_heads, _p(ws), ws_bytes, out.ptr, stream))
+
+
+def page_bounds(pages: KvPages, table: PageTable, layer: int, start: DeviceArray, end: DeviceArray, n: int,
+                bounds: DeviceArray, slots: DeviceArray | None = None, stream=None) -> None:
+    check(lib().lkhip_page_bounds(pages._ref, table._ref, layer, _p(slots), start.ptr, end.ptr, n, bounds.ptr, stream))
+
+
+def sparse_attn_workspace(pages: KvPages, table: PageTable, n: int, n_heads: int, n_take: int) -> int:
+    b = C.c_size_t()
+    check(lib().lkhip_sparse_attn_workspace(pages._ref, table._ref, n, n_heads, n_take, C.byref(b)))
+    return b.value
+
+
+def sparse_attn(pages: KvPages, table: PageTable, layer: int, q: DeviceArray, ctx_len: DeviceArray,
+                bounds: DeviceArray, n: int, n_heads: int, n_take: int, n_first: int, n_last: int, taken: DeviceArray,
+                ws: DeviceArray, ws_bytes: int, out: DeviceArray, slots: DeviceArray | None = None,
+                stream=None) -> None:
+    """One token per sequence over n_take pages of its context; taken gets their numbers."""
+    check(lib().lkhip_sparse_attn(pages._ref, table._ref, layer, q.ptr, _p(slots), ctx_len.ptr, bounds.ptr, n, n_heads,
+                                  n_take, n_first, n_last, taken.ptr, _p(ws), ws_bytes, out.ptr, stream))
 
 
 def memset(d: DeviceArray, value: int) -> None:
