@@ -1,0 +1,259 @@
+// page_choose.hip -- the pages that a sparse attention reads (pages.h LkSparse):
+// scores of a sequence's pages from the bounds of their keys, and the choice.
+#include "lkhip_common.h"
+#include "pages.h"
+
+namespace {
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// A number as an unsigned key of the same order, NaN above all.
+__device__ __forceinline__ uint64_t order_key(double x) {
+    if (x != x) return ~0ull;
+    const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);  // -0 as 0
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+
+// score(page) = max over the kv head's query heads of sum_d max(q_d lo_d, q_d hi_d),
+// which no q.k of the page exceeds; products of f32 and f16 are exact in 64 bits and
+// their sums wrong by 2^-52, so that which page is taken does not hang on the order of
+// a sum (f64 products run at the f32 rate here).  Eight lanes take a page, E = HD / 8
+// dims each; which bound a dim needs hangs on its q alone.
+template <int N>
+__device__ __forceinline__ double dpp_add(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, N, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), N, 0xF, 0xF, false);
+    return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// over eight neighbouring lanes: quad pairs, quad halves, the half row mirrored
+__device__ __forceinline__ double sum8(double x) { return dpp_add<0x141>(dpp_add<0x4E>(dpp_add<0xB1>(x))); }
+
+template <typename KV, int HD>
+struct PageBounds {
+    static constexpr int E = HD / 8, W = E * sizeof(KV) / 4;  // words of a lane's lower, and of its upper bounds
+    uint32_t lo[W], hi[W];
+    __device__ __forceinline__ void load(const void* bounds, const LkPages& p, uint32_t id, uint32_t kvh, uint32_t c) {
+        const u4* b = (const u4*)((const KV*)bounds + ((size_t)id * p.n_kv + kvh) * 2 * HD + c * E);
+        const u4* t = (const u4*)((const KV*)b + HD);
+#pragma unroll
+        for (int w = 0; w < W / 4; w++) {
+            const u4 x = b[w], y = t[w];
+#pragma unroll
+            for (int e = 0; e < 4; e++) lo[4 * w + e] = x[e], hi[4 * w + e] = y[e];
+        }
+    }
+    // q: the lane's E dims
+    __device__ __forceinline__ double score(const double* q) const {
+        double sum = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const double y = q[e];
+            const bool up = y > 0;
+            float f;
+            if constexpr (sizeof(KV) == 4) f = __uint_as_float(up ? hi[e] : lo[e]);
+            else f = lk_h2f((uint16_t)((up ? hi[e / 2] : lo[e / 2]) >> (16 * (e & 1))));
+            sum = fma(y, (double)f, sum);
+        }
+        return sum8(sum);
+    }
+};
+
+// What a sequence holds, for both kernels below.
+__device__ __forceinline__ uint32_t sparse_held(const LkSparse& a, uint32_t slot, uint32_t s) {
+    if (slot >= a.t.n_seq) return 0;
+    const uint32_t cap = a.t.max_pages << a.p.pshift, ctx = a.ctx[s] < cap ? a.ctx[s] : cap;  // < 2^31
+    return (ctx + (1u << a.p.pshift) - 1) >> a.p.pshift;
+}
+__device__ __forceinline__ bool sparse_forced(const LkSparse& a, uint32_t x, uint32_t held) {
+    return x < a.first || x + a.last >= held;
+}
+
+// Keys of pages x0, x0 + step, .. below x1 for one (sequence, kv head), by groups of 8
+// lanes; put(page, key) runs on one lane of the group.  s_q: kHeads x HD doubles.
+constexpr uint32_t kHeads = 8;
+template <typename KV, int HD, class Put>
+__device__ __forceinline__ void score_pages(const LkSparse& a, uint32_t s, uint32_t slot, uint32_t kvh, uint32_t held,
+                                            uint32_t x0, uint32_t x1, uint32_t step, double* s_q, Put put) {
+    constexpr int E = HD / 8;
+    const uint32_t c = threadIdx.x & 7;
+    const uint32_t* row = a.t.table + (size_t)slot * a.t.max_pages;
+    for (uint32_t g0 = 0; g0 < a.G; g0 += kHeads) {
+        const uint32_t gn = a.G - g0 < kHeads ? a.G - g0 : kHeads;
+        __syncthreads();  // the last heads' q is read
+        const float* q = a.q + ((size_t)s * a.n_heads + kvh * a.G + g0) * HD;
+        for (uint32_t i = threadIdx.x; i < gn * HD; i += blockDim.x) s_q[i] = q[i];
+        __syncthreads();
+        for (uint32_t x = x0; x < x1; x += step) {
+            if (sparse_forced(a, x, held)) continue;
+            const uint32_t id = row[x];
+            uint64_t key = 0;  // a hole: below all
+            if (id < a.p.n_pages) {
+                PageBounds<KV, HD> b;
+                b.load(a.bounds, a.p, id, kvh, c);
+                for (uint32_t g = 0; g < gn; g++) {
+                    double y[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++) y[e] = s_q[g * HD + c * E + e];
+                    const uint64_t k = order_key(b.score(y));
+                    key = k > key ? k : key;
+                }
+            }
+            if (c == 0) put(x, key, g0 == 0);
+        }
+    }
+}
+
+// Scores alone, of long tables: many blocks a (sequence, kv head).
+template <typename KV, int HD>
+__global__ __launch_bounds__(256) void sparse_score_kernel(const LkSparse a) {
+    __shared__ __align__(16) double s_q[kHeads * HD];
+    const uint32_t kvh = blockIdx.y, s = blockIdx.z, slot = a.slots ? a.slots[s] : s;
+    const uint32_t held = sparse_held(a, slot, s);
+    if (held <= a.take) return;  // uniform: all are taken
+    uint64_t* keys = a.keys + ((size_t)s * a.p.n_kv + kvh) * a.t.max_pages;
+    score_pages<KV, HD>(a, s, slot, kvh, held, blockIdx.x * 32 + threadIdx.x / 8, held, gridDim.x * 32, s_q,
+                        [&](uint32_t x, uint64_t k, bool first) { keys[x] = first || k > keys[x] ? k : keys[x]; });
+}
+
+// The choice: the want-th largest key by bins of 11 bits, from the highest bit in which
+// the pages still in question differ, so that two or three rounds settle it; then the
+// pages above it and the first of those at it, in order: equal keys go to the lowest
+// page.  One workgroup a (sequence, kv head); FUSED: it takes the scores itself and
+// keeps the keys in LDS.  (A thread that walks 256 bins eight times: 62-78 us.)
+constexpr uint32_t kChoose = 1024, kBins = 2048, kFusedPages = 4096;
+template <typename KV, int HD, bool FUSED>
+__global__ __launch_bounds__(kChoose) void sparse_choose_kernel(const LkSparse a) {
+    __shared__ uint32_t s_bin[kBins], s_part[kChoose / 64], s_find[3];
+    __shared__ uint64_t s_and[kChoose / 64], s_or[kChoose / 64];
+    __shared__ uint64_t s_keys[FUSED ? kFusedPages : 1];
+    __shared__ __align__(16) double s_q[FUSED ? kHeads * HD : 1];
+    const uint32_t kvh = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const uint32_t slot = a.slots ? a.slots[s] : s;
+    uint32_t* sel = a.sel + ((size_t)s * a.p.n_kv + kvh) * a.take;
+    const uint32_t held = sparse_held(a, slot, s);
+    if (held <= a.take) {  // uniform
+        for (uint32_t x = tid; x < a.take; x += kChoose) sel[x] = x < held ? x : LK_NO_PAGE;
+        return;
+    }
+    const uint64_t* keys;
+    if constexpr (FUSED) {
+        score_pages<KV, HD>(a, s, slot, kvh, held, tid / 8, held, kChoose / 8, s_q,
+                            [&](uint32_t x, uint64_t k, bool first) { s_keys[x] = first || k > s_keys[x] ? k : s_keys[x]; });
+        keys = s_keys;
+        __syncthreads();
+    } else {
+        keys = a.keys + ((size_t)s * a.p.n_kv + kvh) * a.t.max_pages;
+    }
+    // sum of v over the threads before this one, and over all
+    auto scan = [&](uint32_t v, uint32_t& all) {
+        uint32_t x = v;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t y = __shfl_up(x, d, 64);
+            if ((int)lane >= d) x += y;
+        }
+        __syncthreads();
+        if (lane == 63) s_part[w] = x;
+        __syncthreads();
+        uint32_t before = 0;
+        all = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kChoose / 64; k++) {
+            const uint32_t y = s_part[k];
+            before += k < w ? y : 0;
+            all += y;
+        }
+        return before + x - v;
+    };
+    const uint32_t others = a.take - a.first - a.last;  // first + last <= take < held
+    uint32_t want = others, shift = 63;
+    uint64_t prefix = 0;  // pages in question: key >> shift >> 1 == prefix (shift 63: all)
+    bool any = others > 0;
+    auto asked = [&](uint32_t x, uint64_t k) { return !sparse_forced(a, x, held) && (k >> shift >> 1) == prefix; };
+    while (any) {  // at most 6 rounds of 11 bits
+        uint64_t all1 = ~0ull, any1 = 0;
+        for (uint32_t x = tid; x < held; x += kChoose) {
+            const uint64_t k = keys[x];
+            if (asked(x, k)) all1 &= k, any1 |= k;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) all1 &= __shfl_xor(all1, d, 64), any1 |= __shfl_xor(any1, d, 64);
+        __syncthreads();
+        if (lane == 0) s_and[w] = all1, s_or[w] = any1;
+        for (uint32_t b = tid; b < kBins; b += kChoose) s_bin[b] = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < kChoose / 64; k++) all1 &= s_and[k], any1 |= s_or[k];
+        const uint64_t differ = all1 ^ any1;
+        if (!differ) {  // all in question are equal
+            shift = 0;
+            prefix = any1;
+            break;
+        }
+        const uint32_t top = 63 - __clzll((long long)differ), sh = top > 10 ? top - 10 : 0;
+        for (uint32_t x = tid; x < held; x += kChoose) {
+            const uint64_t k = keys[x];
+            if (asked(x, k)) atomicAdd(&s_bin[(uint32_t)(k >> sh) & (kBins - 1)], 1u);
+        }
+        __syncthreads();
+        // thread t holds the bins 2 t' and 2 t' + 1 counted from the top
+        const uint32_t b1 = kBins - 1 - 2 * tid, c1 = s_bin[b1], c0 = s_bin[b1 - 1];
+        uint32_t total;
+        const uint32_t above = scan(c1 + c0, total);
+        if (above < want && above + c1 + c0 >= want) {  // one thread
+            const bool lower = above + c1 < want;
+            s_find[0] = lower ? b1 - 1 : b1;
+            s_find[1] = lower ? above + c1 : above;
+            s_find[2] = lower ? c0 : c1;
+        }
+        __syncthreads();
+        const uint32_t bin = s_find[0], count = s_find[2];
+        want -= s_find[1];
+        prefix = (any1 >> sh & ~(uint64_t)(kBins - 1)) | bin;  // bits above the bins are common
+        // from here on in question: key >> sh == prefix
+        any = count != want && sh > 0;
+        shift = sh ? sh - 1 : 0;
+        if (!any) {
+            shift = sh;
+            break;
+        }
+        __syncthreads();
+    }
+    // taken: key >> shift above prefix, and the first `want` of those at it
+    uint32_t out = 0, equal = 0;
+    for (uint32_t x0 = 0; x0 < held; x0 += kChoose) {
+        const uint32_t x = x0 + tid;
+        const bool in = x < held, f = in && sparse_forced(a, x, held);
+        const uint64_t k = in && !f && others ? keys[x] >> shift : 0;
+        const bool mine = in && !f && others, same = mine && k == prefix;
+        uint32_t n_same, n_take;
+        const uint32_t e = equal + scan(same, n_same);
+        const bool takes = f || (mine && k > prefix) || (same && e < want);
+        const uint32_t at = out + scan(takes, n_take);
+        if (takes && at < a.take) sel[at] = x;
+        equal += n_same;
+        out += n_take;
+    }
+}
+
+}  // namespace
+
+template <typename KV, int HD>
+static void select_launch(const LkSparse& a, hipStream_t st) {
+    const dim3 pairs(a.p.n_kv, a.n);
+    if (a.t.max_pages <= kFusedPages) {
+        hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, true>), pairs, dim3(kChoose), 0, st, a);
+        return;
+    }
+    uint32_t blocks = 2048 / (a.n * a.p.n_kv) + 1;
+    const uint32_t most = (a.t.max_pages + 31) / 32;
+    if (blocks > most) blocks = most;
+    hipLaunchKernelGGL((sparse_score_kernel<KV, HD>), dim3(blocks, a.p.n_kv, a.n), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, false>), pairs, dim3(kChoose), 0, st, a);
+}
+hipError_t lk_sparse_select_launch(const LkSparse& a, hipStream_t st) {
+    if (a.p.f32) a.p.hd == 64 ? select_launch<float, 64>(a, st) : select_launch<float, 128>(a, st);
+    else a.p.hd == 64 ? select_launch<uint16_t, 64>(a, st) : select_launch<uint16_t, 128>(a, st);
+    return hipGetLastError();
+}

@@ -7,29 +7,32 @@
 // over the positions x that the row sees, in one pass with running m and sum.
 // All T * G rows of a kv head (T tokens, G query heads) share its K and V.
 //
-// A wave takes RT tiles of 16 rows over tiles of 64 (f32 cache: 32) positions;
-// WR waves of a workgroup lie side by side in rows, the others take positions
-// in turn, and the workgroup one chunk of positions.  Both products run on the
-// matrix cores:
-//   scores S[position][row] = K Q^T: K rows straight from memory as the first
-//     operand (lane: position lane & 15, 8 dims), Q as the second;
+// A wave takes RT tiles of 16 rows over steps of NT tiles of 16 positions.  Both
+// products run on the matrix cores:
+//   scores S[position][row] = K Q^T: K rows are the first operand (lane: position
+//     lane & 15, 8 dims), Q the second;
 //   O[row][dim] += P V: S's lanes hold row lane & 15, positions 4 (lane >> 4) + i
 //     of each 16, which is the first operand of the second product once its k
 //     index is taken as those positions; V is read with the same positions and
-//     HD / 16 neighbouring dims per lane, column n of product d being dim
-//     (HD / 16) n + d, so O's lanes hold neighbouring dims.
-// No operand goes through LDS.  q carries log2(e) / sqrt(hd).  f16 cache: K and V
-// are exact operands; q (scaled per row by a power of two, so that its largest value is in 2^13..2^14) and P
-// are each split into two f16 parts (22 bits), as one part alone is off by
-// 1.4e-4.  f32 cache: 16x16x4 f32 products.
+//     neighbouring dims per lane, so O's lanes hold neighbouring dims.
+// q carries log2(e) / sqrt(hd).  f16 cache: K and V are exact operands; q (scaled
+// per row by a power of two, so that its largest value is in 2^13..2^14) and P are
+// each split into two f16 parts (22 bits), as one part alone is off by 1.4e-4.
+// f32 cache: 16x16x4 f32 products.
 // The running maximum lags: it moves when some score passes it by 8 (in log2),
-// so most tiles neither reduce over lanes nor rescale O; P stays below 2^8.
+// so most steps neither reduce over lanes nor rescale O; P stays below 2^8.
 //
-// Positions that no row sees (behind the draft, in holes of the table) are
-// clamped to readable rows; their scores become -inf and their V zero, so what
-// lies there -- NaN too -- does not matter.  A draft position whose V is not
-// finite would reach the rows that do not see it as 0 * NaN: such a tile takes
-// its V with those values zeroed and then marks (row, dim) pairs that do see one.
+// Two kernels.  Up to 32 rows (narrow): the four waves of a workgroup take steps in
+// turn, K and V go straight from memory to registers, the next step's while this
+// one's are used, and the waves join at the end.  More rows (wide): the waves lie
+// side by side in rows and share each step's K and V through LDS, a ring of stages
+// that loads write without registers.
+//
+// Positions that no row sees (behind the draft, in holes of the table) are clamped
+// to readable rows; their scores become -inf and their V zero, so what lies there
+// -- NaN too -- does not matter.  A draft position whose V is not finite would
+// reach the rows that do not see it as 0 * NaN: such a step takes its V with those
+// values zeroed and then marks the (row, dim) pairs that do see one.
 //
 // A chunk's rows go out as (m, sum, O) and paged_fold_kernel joins them; where a
 // sequence has one chunk its workgroup writes the output itself.
@@ -44,21 +47,14 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLag = 8.f;  // log2: how far a score may pass the running maximum
+constexpr uint32_t kMaxChunks = 64;
 
-__device__ __forceinline__ h8 bits_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __builtin_bit_cast(h8, u4{a, b, c, d});
-}
-__device__ __forceinline__ bool half_not_finite(uint32_t w) {  // either half of w
-    return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
-}
-// w with its non-finite halves as 1.0 and the others 0 (mark), or as 0 and the others kept (clean)
-__device__ __forceinline__ uint32_t half_mark(uint32_t w) {
-    return ((w & 0x7C00u) == 0x7C00u ? 0x3C00u : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0x3C000000u : 0u);
-}
-__device__ __forceinline__ uint32_t half_clean(uint32_t w) {
-    return ((w & 0x7C00u) == 0x7C00u ? 0u : w & 0xFFFFu) | ((w & 0x7C000000u) == 0x7C000000u ? 0u : w & 0xFFFF0000u);
-}
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
+// bits 15 and 31: whether that half of w is not finite
+__device__ __forceinline__ uint32_t halves_not_finite(uint32_t w) {
+    return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+}
+__device__ __forceinline__ uint64_t low_bits(int64_t n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 // What a sequence shows: table row, context and drafted tokens, positions in all.
 struct Seq {
@@ -91,581 +87,665 @@ __device__ __forceinline__ uint32_t chunks_of(uint32_t total, uint32_t chunk) {
     return c ? c : 1;
 }
 
-template <int HD, bool F32, int RT, int WR, bool SPARSE>
-__global__ __launch_bounds__(256) void paged_attn_kernel(const LkPagedAttn a) {
-    constexpr int WP = 4 / WR;           // waves that share a row group's positions
-    constexpr int NT = F32 ? 2 : 4;      // 16-position tiles of a step
-    constexpr int ND = HD / 16;          // column tiles of O, neighbouring dims of a lane
-    constexpr int KS = HD / 32;          // f16 score products of a tile
-    constexpr int ROWS = WR * RT * 16;   // rows of the workgroup
-    __shared__ float s_m[WP][ROWS], s_l[WP][ROWS];
-    __shared__ __align__(16) float s_o[WP > 1 ? ROWS : 1][WP > 1 ? HD + 4 : 1];
-
-    // Row groups of one (sequence, kv head, chunk) read the same K and V: they run
-    // on one XCD (workgroups go round the 8), one after the other.
+// A workgroup's share: one chunk of a (sequence, kv head)'s positions and one group of its rows.  Row groups of one
+// chunk read the same K and V: they run on one XCD (workgroups go round the 8), one after the other.
+struct Share {
+    uint32_t s, kvh, pair, chunk, row0, R, x0, x1, nch;
+    Seq sq;
+    bool live;
+};
+template <bool SPARSE>
+__device__ __forceinline__ Share share_of(const LkPagedAttn& a, uint32_t rows) {
+    Share h{};
     const uint32_t xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
     const uint32_t rg = turn % a.n_rg, item = turn / a.n_rg * 8 + xcd;
-    if (item >= a.n * a.p.n_kv * a.n_chunks) return;
-    const uint32_t chunk = item % a.n_chunks, pair = item / a.n_chunks, kvh = pair % a.p.n_kv, s = pair / a.p.n_kv;
-    const Seq sq = seq_of<SPARSE>(a, s);
-    const uint32_t R = sq.rows * a.G, row0 = rg * ROWS;
-    const uint32_t x0 = chunk * a.chunk;
-    if (!sq.live || row0 >= R || (x0 >= sq.total && chunk)) return;  // uniform
-    const uint32_t nch = chunks_of(sq.total, a.chunk);
-    const uint32_t x1 = x0 + a.chunk < sq.total ? x0 + a.chunk : sq.total;
+    if (item >= a.n * a.p.n_kv * a.n_chunks) return h;
+    h.chunk = item % a.n_chunks;
+    h.pair = item / a.n_chunks;
+    h.kvh = h.pair % a.p.n_kv;
+    h.s = h.pair / a.p.n_kv;
+    h.sq = seq_of<SPARSE>(a, h.s);
+    h.R = h.sq.rows * a.G;
+    h.row0 = rg * rows;
+    h.x0 = h.chunk * a.chunk;
+    h.live = h.sq.live && h.row0 < h.R && (h.x0 < h.sq.total || h.chunk == 0);
+    h.nch = chunks_of(h.sq.total, a.chunk);
+    h.x1 = h.x0 + a.chunk < h.sq.total ? h.x0 + a.chunk : h.sq.total;
+    return h;
+}
 
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t wr = (uint32_t)w % WR, wp = (uint32_t)w / WR;
-    const uint32_t j = (uint32_t)lane >> 4, c16 = (uint32_t)lane & 15;
-    const uint32_t rbase = row0 + wr * (RT * 16);
-    const uint32_t pmask = (1u << a.p.pshift) - 1;
-    const uint32_t* trow = a.t.table + (size_t)sq.slot * a.t.max_pages;
-    const uint32_t* sel = SPARSE ? a.sel + ((size_t)s * a.p.n_kv + kvh) * a.take : nullptr;
-    const uint64_t hoff = kvh * a.p.head_stride;
+// A tile's page id (LK_NO_PAGE or above: a hole) and the sequence position of its first row; y: its place among the
+// positions shown, a multiple of 16.
+template <bool SPARSE>
+__device__ __forceinline__ uint32_t tile_page(const LkPagedAttn& a, const Share& h, uint32_t y, uint32_t& pos) {
+    uint32_t pg = y >> a.p.pshift;
+    bool hole = y >= h.sq.total;
+    if constexpr (SPARSE) {
+        pg = hole ? LK_NO_PAGE : a.sel[((size_t)h.s * a.p.n_kv + h.kvh) * a.take + pg];
+        hole = pg >= a.t.max_pages;
+    }
+    pos = hole ? 0x7FFFFFF0u : (pg << a.p.pshift) + (y & ((1u << a.p.pshift) - 1));
+    return hole ? LK_NO_PAGE : a.t.table[(size_t)h.sq.slot * a.t.max_pages + pg];
+}
+// element of the tile's first row, in the clamped place of a hole
+__device__ __forceinline__ uint64_t tile_base(const LkPagedAttn& a, const Share& h, uint32_t id, uint32_t y, int hd) {
+    return (id < a.p.n_pages ? id * a.p.page_stride + (uint64_t)(y & ((1u << a.p.pshift) - 1)) * hd : 0) +
+           h.kvh * a.p.head_stride;
+}
 
-    // ---- this lane's row of each tile: q and its score factor
+// Dim d (0..HD / 16 - 1) of lane column c16 in the second product.
+template <int HD, bool F32>
+__device__ __forceinline__ constexpr uint32_t dim_of(uint32_t c16, int d) {
+    return F32 ? (d / 4) * 64 + 4 * c16 + d % 4 : HD / 16 * c16 + d;
+}
+
+// A wave's RT tiles of 16 rows: their queries, running maxima and sums, and O.
+template <int HD, bool F32, int RT, int NT, bool SPARSE>
+struct Rows {
+    static constexpr int ND = HD / 16, KS = HD / 32, ES = F32 ? 4 : 2;
+    static constexpr int VW = ND * ES / 4;  // words of a lane's dims of one V row
     h8 qh[F32 ? 1 : RT][F32 ? 1 : KS], ql[F32 ? 1 : RT][F32 ? 1 : KS];
     f4 qf[F32 ? RT : 1][F32 ? ND : 1];
-    float fac[RT];
+    float fac[RT], m[RT], l[RT];
     uint32_t tok[RT];
-    float m[RT], l[RT];
     f4 o[RT][ND];
+    f4 sc[RT][NT];
+    uint32_t j, c16;
+
+    __device__ __forceinline__ void init(const LkPagedAttn& a, const Share& h, uint32_t rbase) {
+        j = (threadIdx.x & 63) >> 4, c16 = threadIdx.x & 15;
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const uint32_t row = rbase + rt * 16 + c16;
-        const bool live = row < R;
-        tok[rt] = live ? row / a.G : 0;
-        const uint32_t g = live ? row % a.G : 0;
-        const float* q = a.q + (((size_t)s * a.tokens + tok[rt]) * a.n_heads + kvh * a.G + g) * HD;
-        m[rt] = -INFINITY;
-        l[rt] = 0.f;
+        for (int rt = 0; rt < RT; rt++) {
+            const uint32_t row = rbase + rt * 16 + c16;
+            const bool live = row < h.R;
+            tok[rt] = live ? row / a.G : 0;
+            const uint32_t g = live ? row - tok[rt] * a.G : 0;
+            const float* q = a.q + (((size_t)h.s * a.tokens + tok[rt]) * a.n_heads + h.kvh * a.G + g) * HD;
+            m[rt] = -INFINITY;
+            l[rt] = 0.f;
 #pragma unroll
-        for (int d = 0; d < ND; d++) o[rt][d] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int d = 0; d < ND; d++) o[rt][d] = f4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (F32) {
+                fac[rt] = 1.f;
+#pragma unroll
+                for (int b = 0; b < ND; b++) {  // dims 16 b + 4 j + e
+                    const f4 x = *(const f4*)(q + 16 * b + 4 * j);
+                    qf[rt][b] = live ? x * a.scale : f4{0.f, 0.f, 0.f, 0.f};
+                }
+            } else {
+                float x[KS][8], top = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {  // dims 32 ks + 8 j + e
+                    const f4 u = *(const f4*)(q + 32 * ks + 8 * j), v = *(const f4*)(q + 32 * ks + 8 * j + 4);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[ks][e] = live ? (e < 4 ? u[e & 3] : v[e & 3]) * a.scale : 0.f;
+                        top = fmaxf(top, fabsf(x[ks][e]));
+                    }
+                }
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                int up = 0;
+                if (top > 0.f && top < INFINITY) {
+                    up = 13 + 127 - (int)((__float_as_uint(top) >> 23) & 255);
+                    up = up > 100 ? 100 : up;  // subnormal rows
+                }
+                fac[rt] = ldexpf(1.f, -up);
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float y = ldexpf(x[ks][e], up);
+                        const _Float16 hi = (_Float16)y;
+                        qh[rt][ks][e] = hi;
+                        ql[rt][ks][e] = (_Float16)(y - (float)hi);
+                    }
+            }
+        }
+    }
+
+    // K operand: f16 the lane's 8 dims 32 ks + 8 j of position c16, f32 its 4 dims 16 b + 4 j
+    __device__ __forceinline__ void scores(int t, int ks, u4 k) {
         if constexpr (F32) {
-            fac[rt] = 1.f;
+            const f4 kk = __builtin_bit_cast(f4, k);
 #pragma unroll
-            for (int b = 0; b < ND; b++) {  // dims 16 b + 4 j + e
-                const float4 x = *(const float4*)(q + 16 * b + 4 * j);
-                qf[rt][b] = live ? f4{x.x, x.y, x.z, x.w} * a.scale : f4{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+                    sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], qf[rt][ks][e], ks == 0 && e == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sc[rt][t], 0, 0, 0);
+        } else {
+            const h8 kk = __builtin_bit_cast(h8, k);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+                sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[rt][ks], ks == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sc[rt][t], 0, 0, 0);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+                sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[rt][ks], sc[rt][t], 0, 0, 0);
+        }
+    }
+
+    // What row c16 of tile rt sees of the step at x: a bit a position.  live: positions that any row may see.
+    __device__ __forceinline__ uint64_t sees(const LkPagedAttn& a, const Share& h, uint32_t x, uint64_t live, int rt) const {
+        if constexpr (SPARSE) return live;
+        const int64_t off = (int64_t)x - h.sq.ctx;  // of the step in the draft
+        uint64_t draft;
+        if (a.mask) {
+            const int32_t words = (int32_t)((a.tokens + 31) / 32), w0 = off >= 0 ? (int32_t)(off >> 5) : 0;
+            const uint32_t* row = a.mask + ((size_t)h.s * a.tokens + tok[rt]) * words;
+            const uint64_t b0 = w0 < words ? row[w0] : 0, b1 = w0 + 1 < words ? row[w0 + 1] : 0,
+                           b2 = w0 + 2 < words ? row[w0 + 2] : 0;
+            if (off >= 0) {
+                const uint32_t sh = off & 31;
+                draft = (b0 | b1 << 32) >> sh;
+                if (sh) draft |= b2 << (64 - sh);
+            } else {
+                draft = off > -64 ? (b0 | b1 << 32) << -off : 0;
             }
         } else {
-            float x[KS][8], top = 0.f;
+            draft = low_bits((int64_t)tok[rt] + 1 - off);
+        }
+        return live & (low_bits(-off) | draft);
+    }
+    __device__ __forceinline__ void hide(int rt, uint64_t see) {
+        const uint32_t b[2] = {(uint32_t)see >> (4 * j), (uint32_t)(see >> 32) >> (4 * j)};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {  // dims 32 ks + 8 j + e
-                const float4 u = *(const float4*)(q + 32 * ks + 8 * j), v = *(const float4*)(q + 32 * ks + 8 * j + 4);
-                const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    x[ks][e] = live ? y[e] * a.scale : 0.f;
-                    top = fmaxf(top, fabsf(x[ks][e]));
-                }
-            }
+            for (int i = 0; i < 4; i++) sc[rt][t][i] = b[t / 2] >> (16 * (t & 1) + i) & 1 ? sc[rt][t][i] : -INFINITY;
+    }
+
+    // Scores become weights; running maximum and sum.
+    __device__ __forceinline__ void weigh(int rt) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) top = fmaxf(top, sc[rt][t][i]);
+        top *= fac[rt];  // a power of two
+        if (__any(top > m[rt] + kLag)) {
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            int up = 0;
-            if (top > 0.f && top < INFINITY) {
-                up = 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127;
-                up = up > 100 ? 100 : up;  // subnormal rows
+            const float mn = fmaxf(m[rt], top);
+            const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - mn);
+            m[rt] = mn;
+            l[rt] *= f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float fi = __shfl(f, (int)(4 * j + i), 64);  // O's rows are 4 j + i
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[rt][d][i] *= fi;
             }
-            fac[rt] = ldexpf(1.f, -up);
+        }
+        const float ms = m[rt] == -INFINITY ? 0.f : m[rt];  // no score yet: weights of 0
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(sc[rt][t][i], fac[rt], -ms));
+                sc[rt][t][i] = p;
+                l[rt] += p;
+            }
+    }
+
+    // v[i]: the lane's dims of position 4 j + i.  f16: two tiles 2 g, 2 g + 1 at once (v, w)
+    __device__ __forceinline__ void add16(int g, const uint32_t (&v)[4][VW], const uint32_t (&w)[4][VW]) {
+        h8 ph[RT], pl[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float p = sc[rt][2 * g + t][i];
+                    const _Float16 hi = (_Float16)p;
+                    ph[rt][4 * t + i] = hi;
+                    pl[rt][4 * t + i] = (_Float16)(p - (float)hi);
+                }
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const uint32_t pick = (d & 1) ? 0x07060302u : 0x05040100u;  // halves d of two positions
+            const h8 vb = __builtin_bit_cast(
+                h8, u4{__builtin_amdgcn_perm(v[1][d / 2], v[0][d / 2], pick), __builtin_amdgcn_perm(v[3][d / 2], v[2][d / 2], pick),
+                       __builtin_amdgcn_perm(w[1][d / 2], w[0][d / 2], pick), __builtin_amdgcn_perm(w[3][d / 2], w[2][d / 2], pick)});
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[rt], vb, o[rt][d], 0, 0, 0);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[rt], vb, o[rt][d], 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void add32(int t, int i, const uint32_t (&v)[VW]) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[rt][t][i], __uint_as_float(v[d % VW]), o[rt][d], 0, 0, 0);
+    }
+
+    // In a masked step: V of positions that no row sees becomes zero, and what is not finite too; the result says
+    // whether there was any.
+    __device__ __forceinline__ uint32_t clean(int t, int i, uint64_t live, uint32_t (&v)[VW]) const {
+        const bool see = live >> (16 * t + 4 * j + i) & 1;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int d = 0; d < VW; d++) {
+            uint32_t y = see ? v[d] : 0;
+            if constexpr (!SPARSE) {
+                if constexpr (F32) {
+                    const bool bad = not_finite(__uint_as_float(y));
+                    odd |= bad;
+                    y = bad ? 0 : y;
+                } else {
+                    const uint32_t bad = halves_not_finite(y);
+                    odd |= bad;
+                    y &= ~((bad >> 15) * 0xFFFFu);
+                }
+            }
+            v[d] = y;
+        }
+        return odd;
+    }
+    // Rows that see a value that is not finite: NaN in its dim.  Rare, so short: a position at a time.
+    __device__ void poison(const LkPagedAttn& a, const Share& h, uint32_t x, uint64_t live) {
+        for (uint32_t p = 0; p < NT * 16; p++) {
+            if (!(live >> p & 1)) continue;  // uniform
+            uint32_t pos;
+            const uint32_t y = x + (p & ~15u), id = tile_page<SPARSE>(a, h, y, pos);
+            const uint64_t at = tile_base(a, h, id, y, HD) + (uint64_t)(p & 15) * HD;
+            uint32_t bad = 0;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const uint64_t e = at + dim_of<HD, F32>(c16, d);
+                bool b;
+                if constexpr (F32) b = not_finite(((const float*)a.p.v)[e]);
+                else b = (((const uint16_t*)a.p.v)[e] & 0x7C00) == 0x7C00;
+                bad |= (uint32_t)b << d;
+            }
+            if (!__any(bad)) continue;
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const uint32_t see = sees(a, h, x, live, rt) >> p & 1;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t hit = __shfl(see, (int)(4 * j + i), 64) ? bad : 0;
+#pragma unroll
+                    for (int d = 0; d < ND; d++) o[rt][d][i] = hit >> d & 1 ? NAN : o[rt][d][i];
+                }
+            }
+        }
+    }
+
+    // row sums over the lanes that share a row
+    __device__ __forceinline__ void close() {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            l[rt] += __shfl_xor(l[rt], 16, 64);
+            l[rt] += __shfl_xor(l[rt], 32, 64);
+        }
+    }
+    // Row lr of the workgroup: the output where the sequence has one chunk, else the chunk's (m, sum, O).
+    __device__ __forceinline__ void put(const LkPagedAttn& a, const Share& h, uint32_t lr, float top, float sum, float (&y)[ND]) const {
+        const uint32_t row = h.row0 + lr;
+        if (row >= h.R) return;
+        float* to;
+        if (h.nch == 1) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: zeros
+#pragma unroll
+            for (int d = 0; d < ND; d++) y[d] *= inv;
+            const uint32_t t = row / a.G;
+            to = a.out + (((size_t)h.s * a.tokens + t) * a.n_heads + h.kvh * a.G + row - t * a.G) * HD;
+        } else {
+            const size_t at = ((size_t)h.pair * a.n_chunks + h.chunk) * a.rows_pad + row;
+            if (c16 == 0) *(float2*)(a.part_ml + 2 * at) = float2{top, sum};
+            to = a.part_o + at * HD;
+        }
+#pragma unroll
+        for (int d = 0; d < ND; d += 4) *(f4*)(to + dim_of<HD, F32>(c16, d)) = f4{y[d], y[d + 1], y[d + 2], y[d + 3]};
+    }
+};
+
+// ---------------------------------------------------------------- narrow
+
+template <int HD, bool F32, int RT, bool SPARSE>
+__global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) {
+    constexpr int NT = F32 || HD == 128 ? 2 : 4, W = 4, ROWS = RT * 16, STEP = NT * 16;
+    using Wave = Rows<HD, F32, RT, NT, SPARSE>;
+    constexpr int ND = Wave::ND, KS = F32 ? ND : Wave::KS, VW = Wave::VW, ES = Wave::ES;
+    __shared__ float s_m[W][ROWS], s_l[W][ROWS];
+    __shared__ __align__(16) float s_o[ROWS][HD + 4];
+    const Share h = share_of<SPARSE>(a, ROWS);
+    if (!h.live) return;  // uniform
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Wave r;
+    u4 kr[2][NT][KS];
+    uint32_t vr[2][NT][4][VW];
+    // a step's tiles: loads go out for all of its K and V
+    auto fetch = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t& live, bool& masked) {
+        const uint32_t j = (threadIdx.x & 63) >> 4, c16 = threadIdx.x & 15;
+        live = 0;
+        masked = false;
+        const char* kb[NT];
+        const char* vb[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            uint32_t pos;
+            const uint32_t y = x + 16 * t, id = tile_page<SPARSE>(a, h, y, pos);
+            const uint64_t base = tile_base(a, h, id, y, HD) * ES;
+            kb[t] = (const char*)a.p.k + base, vb[t] = (const char*)a.p.v + base;
+            const uint32_t end = SPARSE ? h.sq.ctx : h.sq.total;
+            if (id < a.p.n_pages) live |= (low_bits((int64_t)end - pos) & 0xFFFF) << (16 * t);
+            masked |= id >= a.p.n_pages || pos + 16 > h.sq.ctx;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
+                k[t][ks] = *(const u4*)(kb[t] + (c16 * HD * ES + (4 * ks + j) * 16));
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float y = ldexpf(x[ks][e], up);
-                    const _Float16 hi = (_Float16)y;
-                    qh[rt][ks][e] = hi;
-                    ql[rt][ks][e] = (_Float16)(y - (float)hi);
-                }
-        }
-    }
-
-    if (rbase < R) {  // wave-uniform
-        for (uint32_t x = x0 + wp * (NT * 16); x < x1; x += WP * (NT * 16)) {
-            // ---- where the step's 16-position tiles lie
-            uint64_t base[NT];   // element of the tile's first row
-            uint32_t pos[NT];    // its position in the sequence
-            bool hole[NT];
-            bool masked = false;
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const uint32_t y = x + 16 * t;
-                uint32_t pg = y >> a.p.pshift;
-                hole[t] = y >= sq.total;
-                if constexpr (SPARSE) {
-                    pg = hole[t] ? LK_NO_PAGE : sel[pg];
-                    hole[t] = pg >= a.t.max_pages;
-                }
-                const uint32_t id = hole[t] ? LK_NO_PAGE : trow[pg];
-                hole[t] = id >= a.p.n_pages;
-                pos[t] = hole[t] ? 0 : (pg << a.p.pshift) + (y & pmask);
-                base[t] = (hole[t] ? 0 : id * a.p.page_stride + (uint64_t)(y & pmask) * HD) + hoff;
-                masked |= hole[t] || pos[t] + 16 > sq.ctx;
-            }
-            masked = __builtin_amdgcn_readfirstlane(masked);
-            // in a masked step: which of the lane's positions (4 j + i of tile t) no row sees
-            uint32_t unseen = 0;
-            if (masked) {
+            for (int i = 0; i < 4; i++) {
+                const char* row = vb[t] + (4 * j + i) * HD * ES;
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                for (int d = 0; d < ND; d += 16 / ES < ND ? 16 / ES : ND) {
+                    const char* at = row + dim_of<HD, F32>(c16, d) * ES;
+                    if constexpr (VW == 2) {
+                        const u2 y = *(const u2*)at;
+                        v[t][i][0] = y[0], v[t][i][1] = y[1];
+                    } else {
+                        const u4 y = *(const u4*)at;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t y = pos[t] + 4 * j + i;
-                        if (hole[t] || y >= (SPARSE ? sq.ctx : sq.total)) unseen |= 1u << (4 * t + i);
-                    }
-            }
-            auto hide = [&](int rt, int t, int i, float v) -> float {
-                bool see = !(unseen >> (4 * t + i) & 1);
-                if constexpr (!SPARSE) {
-                    const uint32_t y = pos[t] + 4 * j + i;
-                    if (see && y >= sq.ctx) {
-                        const uint32_t d = y - sq.ctx;
-                        if (a.mask) {
-                            const uint32_t words = (a.tokens + 31) / 32;
-                            see = a.mask[((size_t)s * a.tokens + tok[rt]) * words + (d >> 5)] >> (d & 31) & 1;
-                        } else {
-                            see = d <= tok[rt];
-                        }
-                    }
-                }
-                return see ? v : -INFINITY;
-            };
-            // the running maximum and sum of tile rt's rows; sc becomes the weights
-            auto weigh = [&](int rt, f4(&sc)[NT]) {
-                if (masked) {
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) sc[t][i] = hide(rt, t, i, sc[t][i]);
-                }
-                float top = -INFINITY;
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) top = fmaxf(top, sc[t][i]);
-                top *= fac[rt];  // fac > 0
-                if (__any(top > m[rt] + kLag)) {
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                    top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float mn = fmaxf(m[rt], top);
-                    const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - mn);
-                    m[rt] = mn;
-                    l[rt] *= f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float fi = __shfl(f, (int)(4 * j + i), 64);  // O's rows are 4 j + i
-#pragma unroll
-                        for (int d = 0; d < ND; d++) o[rt][d][i] *= fi;
-                    }
-                }
-                const float ms = m[rt] == -INFINITY ? 0.f : m[rt];  // no score yet: weights of 0
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][i], fac[rt], -ms));
-                        sc[t][i] = p;
-                        l[rt] += p;
-                    }
-            };
-            if constexpr (F32) {
-                const float *K = (const float*)a.p.k, *V = (const float*)a.p.v;
-                f4 sc[RT][NT];
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) sc[rt][t] = f4{0.f, 0.f, 0.f, 0.f};
-                    const float* k = K + base[t] + (size_t)c16 * HD + 4 * j;
-#pragma unroll
-                    for (int b = 0; b < ND; b++) {
-                        const f4 kk = *(const f4*)(k + 16 * b);
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-#pragma unroll
-                            for (int rt = 0; rt < RT; rt++)
-                                sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], qf[rt][b][e], sc[rt][t], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) weigh(rt, sc[rt]);
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const f4* v = (const f4*)(V + base[t] + (size_t)(4 * j + i) * HD + ND * c16);
-                        f4 vv[ND / 4];
-#pragma unroll
-                        for (int d = 0; d < ND / 4; d++) vv[d] = v[d];
-                        bool odd = false;
-                        if (masked) {
-                            if (unseen >> (4 * t + i) & 1)
-#pragma unroll
-                                for (int d = 0; d < ND / 4; d++) vv[d] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int d = 0; d < ND; d++) odd |= not_finite(vv[d / 4][d % 4]);
-                            odd = !SPARSE && __any(odd);
-                        }
-                        if (odd) {
-#pragma unroll
-                            for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                                for (int d = 0; d < ND; d++) {
-                                    const float y = vv[d / 4][d % 4];
-                                    const float sees = hide(rt, t, i, 0.f) == 0.f ? 1.f : 0.f;
-                                    f4 c = __builtin_amdgcn_mfma_f32_16x16x4f32(sees, not_finite(y) ? 1.f : 0.f,
-                                                                                f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                                    for (int e = 0; e < 4; e++)
-                                        if (c[e] > 0.f) o[rt][d][e] = NAN;
-                                }
-#pragma unroll
-                            for (int d = 0; d < ND; d++)
-                                if (not_finite(vv[d / 4][d % 4])) vv[d / 4][d % 4] = 0.f;
-                        }
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                            for (int d = 0; d < ND; d++)
-                                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[rt][t][i], vv[d / 4][d % 4], o[rt][d],
-                                                                                0, 0, 0);
-                    }
-            } else {
-                const uint16_t *K = (const uint16_t*)a.p.k, *V = (const uint16_t*)a.p.v;
-                u4 kr[NT][KS];
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++)
-                        kr[t][ks] = *(const u4*)(K + base[t] + (size_t)c16 * HD + 32 * ks + 8 * j);
-                uint32_t vr[NT][4][ND / 2];  // dims ND c16 .. of position 4 j + i
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint16_t* v = V + base[t] + (size_t)(4 * j + i) * HD + ND * c16;
-                        if constexpr (ND == 4) {
-                            const u2 y = *(const u2*)v;
-                            vr[t][i][0] = y[0], vr[t][i][1] = y[1];
-                        } else {
-                            const u4 y = *(const u4*)v;
-                            vr[t][i][0] = y[0], vr[t][i][1] = y[1], vr[t][i][2] = y[2], vr[t][i][3] = y[3];
-                        }
-                    }
-                bool odd = false;
-                if (masked) {
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int d = 0; d < ND / 2; d++) {
-                                if (unseen >> (4 * t + i) & 1) vr[t][i][d] = 0;
-                                odd |= half_not_finite(vr[t][i][d]);
-                            }
-                    odd = !SPARSE && __any(odd);
-                }
-                // operand of column tile d over tiles 2 g, 2 g + 1: halves d of eight positions
-                auto column = [&](const uint32_t(&y)[NT][4][ND / 2], int g, int d) -> h8 {
-                    const uint32_t sel2 = (d & 1) ? 0x07060302u : 0x05040100u;
-                    uint32_t r[4];
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int i = 0; i < 2; i++)
-                            r[2 * t + i] = __builtin_amdgcn_perm(y[2 * g + t][2 * i + 1][d / 2], y[2 * g + t][2 * i][d / 2],
-                                                                 sel2);
-                    return bits_h8(r[0], r[1], r[2], r[3]);
-                };
-                if (odd) {
-                    uint32_t bad[NT][4][ND / 2];
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int d = 0; d < ND / 2; d++) bad[t][i][d] = half_mark(vr[t][i][d]);
-                    // which rows see a marked position (a weight that underflowed to 0 counts: 0 * NaN)
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                        for (int g = 0; g < NT / 2; g++) {
-                            h8 sees;
-#pragma unroll
-                            for (int t = 0; t < 2; t++)
-#pragma unroll
-                                for (int i = 0; i < 4; i++)
-                                    sees[4 * t + i] = hide(rt, 2 * g + t, i, 0.f) == 0.f ? (_Float16)1.f : (_Float16)0.f;
-#pragma unroll
-                            for (int d = 0; d < ND; d++) {
-                                const f4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(sees, column(bad, g, d),
-                                                                                    f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                    if (c[e] > 0.f) o[rt][d][e] = NAN;
-                            }
-                        }
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int d = 0; d < ND / 2; d++) vr[t][i][d] = half_clean(vr[t][i][d]);
-                }
-                h8 vb[NT / 2][ND];
-#pragma unroll
-                for (int g = 0; g < NT / 2; g++)
-#pragma unroll
-                    for (int d = 0; d < ND; d++) vb[g][d] = column(vr, g, d);
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    f4 sc[NT];
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        f4 c = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int ks = 0; ks < KS; ks++) {
-                            const h8 kk = __builtin_bit_cast(h8, kr[t][ks]);
-                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[rt][ks], c, 0, 0, 0);
-                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[rt][ks], c, 0, 0, 0);
-                        }
-                        sc[t] = c;
-                    }
-                    weigh(rt, sc);
-#pragma unroll
-                    for (int g = 0; g < NT / 2; g++) {
-                        h8 ph, pl;
-#pragma unroll
-                        for (int t = 0; t < 2; t++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const float p = sc[2 * g + t][i];
-                                const _Float16 hi = (_Float16)p;
-                                ph[4 * t + i] = hi;
-                                pl[4 * t + i] = (_Float16)(p - (float)hi);
-                            }
-#pragma unroll
-                        for (int d = 0; d < ND; d++) {
-                            o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vb[g][d], o[rt][d], 0, 0, 0);
-                            o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vb[g][d], o[rt][d], 0, 0, 0);
-                        }
+                        for (int e = 0; e < 4; e++) v[t][i][d * ES / 4 + e] = y[e];
                     }
                 }
             }
-        }
-    }
-
-    // ---- the waves of a row group join: m and sum per row, then O one wave after the other
+    };
+    auto use = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t live, bool masked) {
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        l[rt] += __shfl_xor(l[rt], 16, 64);
-        l[rt] += __shfl_xor(l[rt], 32, 64);
-        if (j == 0) {
-            s_m[wp][wr * (RT * 16) + rt * 16 + c16] = m[rt];
-            s_l[wp][wr * (RT * 16) + rt * 16 + c16] = l[rt];
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) r.scores(t, ks, k[t][ks]);
+        if (__builtin_amdgcn_readfirstlane(masked)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt));
+            uint32_t odd = 0;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) odd |= r.clean(t, i, live, v[t][i]);
+            if (__any(odd)) r.poison(a, h, x, live);
         }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) r.weigh(rt);
+        if constexpr (F32) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) r.add32(t, i, v[t][i]);
+        } else {
+#pragma unroll
+            for (int g = 0; g < NT / 2; g++) r.add16(g, v[2 * g], v[2 * g + 1]);
+        }
+    };
+    uint32_t x = h.x0 + w * STEP;
+    uint64_t live[2];
+    bool masked[2];
+    if (x < h.x1) fetch(x, kr[0], vr[0], live[0], masked[0]);
+    r.init(a, h, h.row0);
+    while (x < h.x1) {
+        uint32_t nx = x + W * STEP;
+        if (nx < h.x1) fetch(nx, kr[1], vr[1], live[1], masked[1]);
+        use(x, kr[0], vr[0], live[0], masked[0]);
+        x = nx;
+        if (x >= h.x1) break;
+        nx = x + W * STEP;
+        if (nx < h.x1) fetch(nx, kr[0], vr[0], live[0], masked[0]);
+        use(x, kr[1], vr[1], live[1], masked[1]);
+        x = nx;
     }
+    // ---- the waves join: m and sum per row, then O one wave after the other
+    r.close();
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+        if (r.j == 0) s_m[w][rt * 16 + r.c16] = r.m[rt], s_l[w][rt * 16 + r.c16] = r.l[rt];
     __syncthreads();
-    const size_t pbase = ((size_t)pair * a.n_chunks + chunk) * a.rows_pad + row0;
-    for (int turn2 = 0; turn2 < WP; turn2++) {
-        if ((int)wp == turn2) {
+    for (uint32_t turn = 0; turn < W; turn++) {
+        if (w == turn) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const uint32_t lr = wr * (RT * 16) + rt * 16 + 4 * j + i, row = row0 + lr;
+                    const uint32_t lr = rt * 16 + 4 * r.j + i;
                     float top = -INFINITY, sum = 0.f;
 #pragma unroll
-                    for (int k = 0; k < WP; k++) top = fmaxf(top, s_m[k][lr]);
+                    for (int k = 0; k < W; k++) top = fmaxf(top, s_m[k][lr]);
                     const float ms = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                    for (int k = 0; k < WP; k++) sum += s_l[k][lr] * __builtin_amdgcn_exp2f(s_m[k][lr] - ms);
-                    const float f = __builtin_amdgcn_exp2f(s_m[wp][lr] - ms);  // 0 for a wave that saw nothing
+                    for (int k = 0; k < W; k++) sum += s_l[k][lr] * __builtin_amdgcn_exp2f(s_m[k][lr] - ms);
+                    const float f = __builtin_amdgcn_exp2f(s_m[w][lr] - ms);  // 0 for a wave that saw nothing
                     float y[ND];
 #pragma unroll
-                    for (int d = 0; d < ND; d++) y[d] = o[rt][d][i] * f;
-                    if constexpr (WP > 1) {
-                        float* acc = &s_o[lr][ND * c16];
-                        if (turn2 > 0)
+                    for (int d = 0; d < ND; d++) y[d] = r.o[rt][d][i] * f;
 #pragma unroll
-                            for (int d = 0; d < ND; d++) y[d] += acc[d];
-                        if (turn2 < WP - 1) {
+                    for (int d = 0; d < ND; d += 4) {
+                        f4* acc = (f4*)&s_o[lr][dim_of<HD, F32>(r.c16, d)];
+                        f4 z = f4{y[d], y[d + 1], y[d + 2], y[d + 3]};
+                        if (turn > 0) z += *acc;
+                        if (turn < W - 1) *acc = z;
 #pragma unroll
-                            for (int d = 0; d < ND; d++) acc[d] = y[d];
-                            continue;
-                        }
+                        for (int e = 0; e < 4; e++) y[d + e] = z[e];
                     }
-                    if (row >= R) continue;
-                    float* to;
-                    if (nch == 1) {
-                        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: zeros
-#pragma unroll
-                        for (int d = 0; d < ND; d++) y[d] *= inv;
-                        to = a.out + (((size_t)s * a.tokens + row / a.G) * a.n_heads + kvh * a.G + row % a.G) * HD;
-                    } else {
-                        if (c16 == 0) *(float2*)(a.part_ml + 2 * (pbase + lr)) = float2{top, sum};
-                        to = a.part_o + (pbase + lr) * HD;
-                    }
-#pragma unroll
-                    for (int d = 0; d < ND; d += 4) *(f4*)(to + ND * c16 + d) = f4{y[d], y[d + 1], y[d + 2], y[d + 3]};
+                    if (turn == W - 1) r.put(a, h, lr, top, sum, y);
                 }
         }
-        if (turn2 < WP - 1) __syncthreads();
+        __syncthreads();
     }
 }
 
-// Chunks of a row, joined: HD / 4 lanes a row.
+// ------------------------------------------------------------------ wide
+
+// NW waves side by side in rows, 32 rows each.  A stage is a step's K, then its V: rows of HD * ES bytes, whose 16-byte
+// pieces lie at their number ^ (row & 7), so that eight lanes that read one piece of eight rows meet eight different
+// bank groups.  Loads write LDS in lane order, so the lane that lands in a place fetches the piece that belongs there.
+template <int HD, bool F32, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void paged_wide_kernel(const LkPagedAttn a) {
+    constexpr int RT = 2, NT = F32 ? 2 : 4, STEP = NT * 16;
+    using Wave = Rows<HD, F32, RT, NT, false>;
+    constexpr int ND = Wave::ND, KS = F32 ? ND : Wave::KS, VW = Wave::VW, ES = Wave::ES;
+    constexpr int RB = HD * ES, PIECES = RB / 16, PER = 64 / PIECES;   // rows that one load instruction covers
+    constexpr int HALF = STEP * RB, STAGE = 2 * HALF, OPS = STAGE / 1024 / NW;
+    constexpr int RING = STAGE <= 16384 ? 3 : 2;
+    static_assert(OPS >= 1 && STAGE % (1024 * NW) == 0 && 16 % PER == 0, "whole load instructions, each within a tile");
+    __shared__ __align__(1024) char ring[RING][STAGE];
+    const Share h = share_of<false>(a, NW * 32);
+    if (!h.live) return;  // uniform
+    const uint32_t lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t rbase = h.row0 + w * 32;
+    const bool busy = rbase < h.R;  // wave-uniform; an idle wave loads with the others
+    const uint32_t steps = (h.x1 - h.x0 + STEP - 1) / STEP;
+
+    // Page ids of the chunk's tiles, 64 at a time, one a lane; `ahead` are the next 64.
+    auto ids_of = [&](uint32_t block) -> uint32_t {
+        uint32_t pos;
+        const uint64_t y = (uint64_t)h.x0 + ((uint64_t)block * 64 + lane) * 16;
+        return y < h.x1 ? tile_page<false>(a, h, (uint32_t)y, pos) : LK_NO_PAGE;
+    };
+    uint32_t ids = ids_of(0), ahead = ids_of(1), block = 0;
+    typedef __attribute__((address_space(3))) uint32_t* lptr;
+    typedef __attribute__((address_space(1))) uint32_t* gptr;
+    auto issue = [&](uint32_t n, char* stage) {
+        const uint32_t x = h.x0 + n * STEP;
+#pragma unroll
+        for (int k = 0; k < OPS; k++) {
+            const uint32_t q = w * OPS + k, row0 = q * PER % STEP;  // the K loads, then the V loads
+            const uint32_t tile = (n * STEP + row0) / 16;
+            const uint32_t id = __builtin_amdgcn_readlane(ids, tile & 63);
+            const uint32_t row = row0 + lane / PIECES, piece = (lane % PIECES) ^ (row & 7);
+            const uint64_t at = tile_base(a, h, id, x + (row0 & ~15u), HD) * ES + (row & 15) * RB + piece * 16;
+            const char* from = (const char*)(q * PER >= STEP ? a.p.v : a.p.k) + at;
+            __builtin_amdgcn_global_load_lds((gptr)from, (lptr)(stage + q * 1024), 16, 0, 0);
+        }
+    };
+    // a step's ids before its issue: the next block of 64 begins every 64 / NT steps
+    auto turn_page = [&](uint32_t n) {
+        if (n * NT / 64 != block) {
+            block++;
+            ids = ahead;
+            ahead = ids_of(block + 1);
+        }
+    };
+    // whether a step has something to hide, and which positions are there, is kept for the RING - 1 steps till its use
+    auto look = [&](uint32_t n, uint64_t& live) -> bool {
+        const uint32_t x = h.x0 + n * STEP;
+        live = 0;
+        bool masked = x + STEP > h.sq.ctx;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const uint32_t id = __builtin_amdgcn_readlane(ids, (n * NT + t) & 63);
+            masked |= id >= a.p.n_pages;
+            if (id < a.p.n_pages) live |= (low_bits((int64_t)h.sq.total - (x + 16 * t)) & 0xFFFF) << (16 * t);
+        }
+        return masked;
+    };
+    Wave r;
+    // of the steps under way: what is there, and whether something is to be hidden
+    uint64_t live[RING - 1];
+    bool masked[RING - 1];
+#pragma unroll
+    for (int n = 0; n < RING - 1; n++) {
+        masked[n] = false, live[n] = 0;
+        if ((uint32_t)n < steps) {
+            masked[n] = look(n, live[n]);
+            issue(n, ring[n]);
+        }
+    }
+    r.init(a, h, rbase);
+    auto scores = [&](const char* stage) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const uint32_t row = 16 * t + r.c16;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) r.scores(t, ks, *(const u4*)(stage + row * RB + ((4 * ks + r.j) ^ (row & 7)) * 16));
+        }
+    };
+    auto value = [&](const char* stage, int t, int i, uint32_t (&v)[VW]) {
+        const uint32_t row = 16 * t + 4 * r.j + i;
+        const char* at = stage + HALF + row * RB;
+        if constexpr (VW == 2) {
+            const u2 y = *(const u2*)(at + ((r.c16 / 2) ^ (row & 7)) * 16 + (r.c16 & 1) * 8);
+            v[0] = y[0], v[1] = y[1];
+        } else {
+#pragma unroll
+            for (int d = 0; d < VW; d += 4) {
+                const u4 y = *(const u4*)(at + ((d * 4 + r.c16) ^ (row & 7)) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[d + e] = y[e];
+            }
+        }
+    };
+    uint32_t slot = 0;  // n % RING
+    for (uint32_t n = 0; n < steps; n++) {
+        // step n has landed for every wave, and every wave is done with the stage that is filled next
+        if (RING > 2 && n + RING - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * OPS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const bool mk = masked[0];
+        const uint64_t lv = live[0];
+#pragma unroll
+        for (int k = 0; k + 1 < RING - 1; k++) masked[k] = masked[k + 1], live[k] = live[k + 1];
+        if (n + RING - 1 < steps) {
+            turn_page(n + RING - 1);
+            masked[RING - 2] = look(n + RING - 1, live[RING - 2]);
+            issue(n + RING - 1, ring[slot ? slot - 1 : RING - 1]);
+        }
+        const char* stage = ring[slot];
+        slot = slot + 1 < RING ? slot + 1 : 0;
+        if (!busy) continue;
+        const uint32_t x = h.x0 + n * STEP;
+        scores(stage);
+        if (mk) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, lv, rt));
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) r.weigh(rt);
+        uint32_t odd = 0;
+        if constexpr (F32) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t v[VW];
+                    value(stage, t, i, v);
+                    if (mk) odd |= r.clean(t, i, lv, v);
+                    r.add32(t, i, v);
+                }
+        } else {
+#pragma unroll
+            for (int g = 0; g < NT / 2; g++) {
+                uint32_t v[2][4][VW];
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) value(stage, 2 * g + t, i, v[t][i]);
+                if (mk) {
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) odd |= r.clean(2 * g + t, i, lv, v[t][i]);
+                }
+                r.add16(g, v[0], v[1]);
+            }
+        }
+        if (mk && __any(odd)) r.poison(a, h, x, lv);
+    }
+    if (!busy) return;  // no barrier follows
+    r.close();
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float y[ND];
+#pragma unroll
+            for (int d = 0; d < ND; d++) y[d] = r.o[rt][d][i];
+            const int from = (int)(4 * r.j + i);  // the lane that holds row 4 j + i's m and sum
+            r.put(a, h, w * 32 + rt * 16 + 4 * r.j + i, __shfl(r.m[rt], from, 64), __shfl(r.l[rt], from, 64), y);
+        }
+}
+
+// Chunks of a row, joined.  A block takes four rows: a wave weighs a row's chunks (lane = chunk, at most 64),
+// then HD / 4 lanes by SPLIT groups a row add them up, each group every SPLIT-th chunk: two dependent reads of
+// memory in all.  (One thread group walking the chunks of a row: 19.6 us for 33 chunks of 112 rows x 8.)
 template <int HD, bool SPARSE>
 __global__ __launch_bounds__(256) void paged_fold_kernel(const LkPagedAttn a) {
-    constexpr uint32_t L = HD / 4;
+    constexpr uint32_t L = HD / 4, SPLIT = 64 / L;
+    __shared__ float s_f[4][kMaxChunks];
+    __shared__ __align__(16) f4 s_y[4][SPLIT][L];
     const uint32_t pair = blockIdx.x, kvh = pair % a.p.n_kv, s = pair / a.p.n_kv;
     const Seq sq = seq_of<SPARSE>(a, s);
-    const uint32_t nch = chunks_of(sq.total, a.chunk);
-    const uint32_t row = blockIdx.y * (256 / L) + threadIdx.x / L, c = threadIdx.x % L;
-    if (!sq.live || nch == 1 || row >= sq.rows * a.G) return;
+    const uint32_t nch = chunks_of(sq.total, a.chunk), R = sq.rows * a.G;
+    if (!sq.live || nch == 1 || blockIdx.y * 4 >= R) return;  // uniform
+    const uint32_t w = threadIdx.x >> 6, lane = threadIdx.x & 63, row = blockIdx.y * 4 + w;
     const size_t base = (size_t)pair * a.n_chunks * a.rows_pad + row;
-    float top = -INFINITY;
-    for (uint32_t k = 0; k < nch; k++) top = fmaxf(top, a.part_ml[2 * (base + (size_t)k * a.rows_pad)]);
-    const float ms = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+    if (row < R) {  // wave-uniform
+        float2 ml{-INFINITY, 0.f};
+        if (lane < nch) ml = *(const float2*)(a.part_ml + 2 * (base + (size_t)lane * a.rows_pad));
+        const float top = lk_wave_max(ml.x), f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
+        const float sum = lk_wave_sum(ml.y * f);
+        s_f[w][lane] = f * (sum == 0.f ? 0.f : 1.f / sum);
+    }
+    __syncthreads();
+    const uint32_t c = lane % L, sp = lane / L;
     f4 y = f4{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t k = 0; k < nch; k++) {
-        const size_t at = base + (size_t)k * a.rows_pad;
-        const float2 ml = *(const float2*)(a.part_ml + 2 * at);
-        const float f = __builtin_amdgcn_exp2f(ml.x - ms);
-        sum = fmaf(ml.y, f, sum);
-        y += *(const f4*)(a.part_o + at * HD + 4 * c) * f;
+    if (row < R) {
+#pragma unroll 4
+        for (uint32_t k = sp; k < nch; k += SPLIT)
+            y += *(const f4*)(a.part_o + (base + (size_t)k * a.rows_pad) * HD + 4 * c) * s_f[w][k];
     }
-    y *= sum == 0.f ? 0.f : 1.f / sum;
+    s_y[w][sp][c] = y;
+    __syncthreads();
+    if (row >= R || sp) return;
+#pragma unroll
+    for (uint32_t k = 1; k < SPLIT; k++) y += s_y[w][k][c];
     *(f4*)(a.out + (((size_t)s * a.tokens + row / a.G) * a.n_heads + kvh * a.G + row % a.G) * HD + 4 * c) = y;
-}
-
-// ------------------------------------------------------------ choosing pages
-
-// A number as an unsigned key of the same order, NaN above all.
-__device__ __forceinline__ uint64_t order_key(double x) {
-    if (x != x) return ~0ull;
-    const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);  // -0 as 0
-    return b >> 63 ? ~b : b | 1ull << 63;
-}
-
-// score(page) = max over the kv head's query heads of sum_d max(q_d lo_d, q_d hi_d),
-// which no q.k of the page exceeds; products of f32 and f16 are exact in 64 bits and
-// their sums wrong by 2^-52, so that which page is taken does not hang on the order of
-// a sum.  A group of 8 lanes takes a page, HD / 8 dims each.
-template <typename KV, int HD>
-__global__ __launch_bounds__(256) void sparse_score_kernel(const LkSparse a) {
-    constexpr int E = HD / 8;
-    const uint32_t kvh = blockIdx.y, s = blockIdx.z;
-    const uint32_t slot = a.slots ? a.slots[s] : s;
-    if (slot >= a.t.n_seq) return;
-    const uint64_t cap = (uint64_t)a.t.max_pages << a.p.pshift;
-    const uint64_t ctx = a.ctx[s] < cap ? a.ctx[s] : cap;
-    const uint32_t held = (uint32_t)((ctx + (1u << a.p.pshift) - 1) >> a.p.pshift);
-    if (held <= a.take) return;  // all are taken
-    const uint32_t pg = blockIdx.x * 32 + threadIdx.x / 8, c = threadIdx.x % 8;
-    if (pg >= held) return;  // whole groups of 8
-    uint64_t key = ~0ull;
-    if (pg >= a.first && pg + a.last < held) {
-        const uint32_t id = a.t.table[(size_t)slot * a.t.max_pages + pg];
-        key = 0;
-        if (id < a.p.n_pages) {
-            const KV* lo = (const KV*)a.bounds + (((size_t)id * a.p.n_kv + kvh) * 2) * HD + c * E;
-            const KV* hi = lo + HD;
-            double bl[E], bh[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                if constexpr (sizeof(KV) == 4) bl[e] = lo[e], bh[e] = hi[e];
-                else bl[e] = lk_h2f(lo[e]), bh[e] = lk_h2f(hi[e]);
-            }
-            const float* q = a.q + ((size_t)s * a.n_heads + kvh * a.G) * HD + c * E;
-            for (uint32_t g = 0; g < a.G; g++) {
-                double sum = 0;
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const double y = q[(size_t)g * HD + e];
-                    sum = fma(y, y > 0 ? bh[e] : bl[e], sum);
-                }
-#pragma unroll
-                for (int d = 1; d < 8; d *= 2) sum += __shfl_xor(sum, d, 64);
-                const uint64_t k = order_key(sum);
-                key = k > key ? k : key;
-            }
-        }
-    }
-    if (c == 0) a.keys[((size_t)s * a.p.n_kv + kvh) * a.t.max_pages + pg] = key;
-}
-
-// The `take` largest keys, equal ones by lowest page: the take-th largest key by its
-// digits of 8 bits from the top (a histogram of the pages that agree so far), then the
-// pages above it and the first of those at it, in order.  First and last pages have
-// the highest key and a NaN score has it too, so it is looked at beside them.
-constexpr uint32_t kSelect = 256;
-__global__ __launch_bounds__(kSelect) void sparse_select_kernel(const LkSparse a) {
-    __shared__ uint32_t hist[256], s_part[kSelect / 64], s_digit, s_above;
-    const uint32_t kvh = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
-    const uint32_t slot = a.slots ? a.slots[s] : s;
-    uint32_t* sel = a.sel + ((size_t)s * a.p.n_kv + kvh) * a.take;
-    const uint64_t cap = (uint64_t)a.t.max_pages << a.p.pshift;
-    const uint64_t ctx = slot < a.t.n_seq ? (a.ctx[s] < cap ? a.ctx[s] : cap) : 0;
-    const uint32_t held = (uint32_t)((ctx + (1u << a.p.pshift) - 1) >> a.p.pshift);
-    if (held <= a.take) {  // uniform
-        for (uint32_t x = tid; x < a.take; x += kSelect) sel[x] = x < held ? x : LK_NO_PAGE;
-        return;
-    }
-    const uint64_t* keys = a.keys + ((size_t)s * a.p.n_kv + kvh) * a.t.max_pages;
-    auto forced = [&](uint32_t x) { return x < a.first || x + a.last >= held; };
-    // first + last <= take (host): what is left for the others
-    const uint32_t want0 = a.take - a.first - a.last;
-    uint32_t want = want0;  // of the pages that agree with `prefix` so far
-    uint64_t prefix = 0, known = 0;
-    for (int shift = 56; shift >= 0 && want; shift -= 8) {
-        hist[tid] = 0;
-        __syncthreads();
-        for (uint32_t x = tid; x < held; x += kSelect)
-            if (!forced(x) && (keys[x] & known) == prefix) atomicAdd(&hist[keys[x] >> shift & 255], 1u);
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t above = 0;
-            int d = 255;
-            while (d > 0 && above + hist[d] < want) above += hist[d--];
-            s_digit = d;
-            s_above = above;
-        }
-        __syncthreads();
-        prefix |= (uint64_t)s_digit << shift;
-        known |= 255ull << shift;
-        want -= s_above;
-        __syncthreads();
-    }
-    // pages above `prefix`, and the first `want` of those equal to it
-    uint32_t out = 0, equal = 0;
-    for (uint32_t x0 = 0; x0 < held; x0 += kSelect) {
-        const uint32_t x = x0 + tid;
-        const bool in = x < held, f = in && forced(x);
-        const uint64_t k = in ? keys[x] : 0;
-        const bool same = in && !f && want0 && k == prefix;
-        auto place = [&](bool v, uint32_t& all) {
-            const uint64_t b = __ballot(v);
-            __syncthreads();
-            if ((tid & 63) == 0) s_part[tid >> 6] = __popcll(b);
-            __syncthreads();
-            uint32_t before = __popcll(b & ((1ull << (tid & 63)) - 1));
-            all = 0;
-            for (uint32_t i = 0; i < kSelect / 64; i++) {
-                if (i < tid >> 6) before += s_part[i];
-                all += s_part[i];
-            }
-            return before;
-        };
-        uint32_t n_same, n_take;
-        const uint32_t e = equal + place(same, n_same);
-        const bool takes = f || (in && want0 && k > prefix) || (same && e < want);
-        const uint32_t at = out + place(takes, n_take);
-        if (takes && at < a.take) sel[at] = x;
-        equal += n_same;
-        out += n_take;
-    }
 }
 
 }  // namespace
@@ -673,16 +753,17 @@ __global__ __launch_bounds__(kSelect) void sparse_select_kernel(const LkSparse a
 LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32_t n_kv, uint32_t rows,
                           uint64_t positions) {
     LkPagedPlan p{};
-    p.rt = sparse || rows <= 16 ? 1 : rows <= 32 || hd == 128 || f32 ? 2 : 4;
-    const uint32_t per = p.rt * 16;
-    p.wr = sparse ? 1 : rows > 2 * per ? 4 : rows > per ? 2 : 1;
-    p.n_rg = (rows + p.wr * per - 1) / (p.wr * per);
-    p.rows_pad = p.n_rg * p.wr * per;
+    p.narrow = sparse || rows <= 32;
+    p.tiles = p.narrow ? (rows <= 16 || sparse ? 1 : 2) : 2;
+    p.waves = p.narrow ? 4 : rows <= 64 ? 2 : 4;
+    const uint32_t per = p.narrow ? p.tiles * 16 : p.waves * 32;
+    p.n_rg = (rows + per - 1) / per;
+    p.rows_pad = p.n_rg * per;
     const uint64_t base = (uint64_t)n * n_kv * p.n_rg;
-    const uint32_t step = 64 * (4 / p.wr);  // every wave has a step
+    const uint32_t step = p.narrow ? (f32 || hd == 128 ? 32 : 64) * 4 : 64;  // narrow: every wave has a step
     const uint64_t steps = (positions + step - 1) / step;
     uint64_t c = (1024 + base - 1) / base;
-    c = c > 64 ? 64 : c;
+    c = c > kMaxChunks ? kMaxChunks : c;
     c = c > steps ? steps : c;
     if (c < 1) c = 1;
     p.chunk = (uint32_t)((steps + c - 1) / c * step);
@@ -698,23 +779,20 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
 template <int HD, bool F32, bool SPARSE>
 static hipError_t launch(const LkPagedAttn& a, const LkPagedPlan& p, hipStream_t st) {
     const dim3 grid((uint32_t)p.blocks);
-#define LK_PAGED(RT, WR) \
-    hipLaunchKernelGGL((paged_attn_kernel<HD, F32, RT, WR, SPARSE>), grid, dim3(256), 0, st, a)
-    constexpr int TOP = HD == 64 && !F32 ? 4 : 2;
-    if constexpr (SPARSE) {
-        if (p.rt != 1 || p.wr != 1) return hipErrorInvalidValue;
-        LK_PAGED(1, 1);
-    } else if (p.rt == 1 && p.wr == 1) LK_PAGED(1, 1);
-    else if (p.rt == 2 && p.wr == 1) LK_PAGED(2, 1);
-    else if (p.rt == TOP && p.wr == 1) LK_PAGED(TOP, 1);
-    else if (p.rt == TOP && p.wr == 2) LK_PAGED(TOP, 2);
-    else if (p.rt == TOP && p.wr == 4) LK_PAGED(TOP, 4);
-    else return hipErrorInvalidValue;
-#undef LK_PAGED
+    if (p.narrow) {
+        if (p.tiles == 1) hipLaunchKernelGGL((paged_narrow_kernel<HD, F32, 1, SPARSE>), grid, dim3(256), 0, st, a);
+        else if (!SPARSE) hipLaunchKernelGGL((paged_narrow_kernel<HD, F32, 2, false>), grid, dim3(256), 0, st, a);
+        else return hipErrorInvalidValue;
+    } else if (SPARSE) {
+        return hipErrorInvalidValue;
+    } else if (p.waves == 2) {
+        hipLaunchKernelGGL((paged_wide_kernel<HD, F32, 2>), grid, dim3(128), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((paged_wide_kernel<HD, F32, 4>), grid, dim3(256), 0, st, a);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.n_chunks == 1) return e;
-    const uint32_t rows = a.tokens * a.G, per = 256 / (HD / 4);
-    hipLaunchKernelGGL((paged_fold_kernel<HD, SPARSE>), dim3(a.n * a.p.n_kv, (rows + per - 1) / per), dim3(256), 0, st,
+    hipLaunchKernelGGL((paged_fold_kernel<HD, SPARSE>), dim3(a.n * a.p.n_kv, (a.tokens * a.G + 3) / 4), dim3(256), 0, st,
                        a);
     return hipGetLastError();
 }
@@ -733,16 +811,4 @@ hipError_t lk_paged_attn_launch(LkPagedAttn a, const LkPagedPlan& p, void* ws, h
     if (a.p.hd == 64) return a.p.f32 ? LK_PAGED(64, true) : LK_PAGED(64, false);
     return a.p.f32 ? LK_PAGED(128, true) : LK_PAGED(128, false);
 #undef LK_PAGED
-}
-
-hipError_t lk_sparse_select_launch(const LkSparse& a, hipStream_t st) {
-    const dim3 grid((a.t.max_pages + 31) / 32, a.p.n_kv, a.n);
-    if (a.t.max_pages > a.take) {
-        if (a.p.f32 && a.p.hd == 64) hipLaunchKernelGGL((sparse_score_kernel<float, 64>), grid, dim3(256), 0, st, a);
-        else if (a.p.f32) hipLaunchKernelGGL((sparse_score_kernel<float, 128>), grid, dim3(256), 0, st, a);
-        else if (a.p.hd == 64) hipLaunchKernelGGL((sparse_score_kernel<uint16_t, 64>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((sparse_score_kernel<uint16_t, 128>), grid, dim3(256), 0, st, a);
-    }
-    hipLaunchKernelGGL(sparse_select_kernel, dim3(a.p.n_kv, a.n), dim3(kSelect), 0, st, a);
-    return hipGetLastError();
 }

@@ -66,7 +66,8 @@ struct LkPagedAttn {
     float scale;           // log2(e) / sqrt(hd)
 };
 struct LkPagedPlan {
-    uint32_t rt, wr;       // 16-row tiles of a wave; waves of a workgroup side by side in rows
+    bool narrow;           // waves take positions in turn; else they lie side by side in rows
+    uint32_t tiles, waves; // 16-row tiles of a wave, waves of a workgroup
     uint32_t chunk, n_chunks, n_rg, rows_pad;
     uint64_t blocks;
     uint64_t part_bytes;
