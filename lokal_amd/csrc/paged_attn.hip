@@ -42,6 +42,7 @@
 namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __fp16 p2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
@@ -290,17 +291,22 @@ struct Rows {
     // v[i]: the lane's dims of position 4 j + i.  f16: two tiles 2 g, 2 g + 1 at once (v, w)
     __device__ __forceinline__ void add16(int g, const uint32_t (&v)[4][VW], const uint32_t (&w)[4][VW]) {
         h8 ph[RT], pl[RT];
+        float minus = -1.f;  // a register: p - hi is then one mixed product, hi not widened first
+        asm("" : "+s"(minus));
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
+        for (int rt = 0; rt < RT; rt++) {
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float p = sc[rt][2 * g + t][i];
-                    const _Float16 hi = (_Float16)p;
-                    ph[rt][4 * t + i] = hi;
-                    pl[rt][4 * t + i] = (_Float16)(p - (float)hi);
-                }
+            for (int e = 0; e < 4; e++) {  // truncated to f16; what that leaves fits f16's 11 bits but for two
+                const float p0 = sc[rt][2 * g + e / 2][2 * (e & 1)], p1 = sc[rt][2 * g + e / 2][2 * (e & 1) + 1];
+                const p2 u = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+                hi[e] = __builtin_bit_cast(uint32_t, u);
+                lo[e] = __builtin_bit_cast(
+                    uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)u[0], minus, p0), __builtin_fmaf((float)u[1], minus, p1)));
+            }
+            ph[rt] = __builtin_bit_cast(h8, u4{hi[0], hi[1], hi[2], hi[3]});
+            pl[rt] = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
+        }
 #pragma unroll
         for (int d = 0; d < ND; d++) {
             const uint32_t pick = (d & 1) ? 0x07060302u : 0x05040100u;  // halves d of two positions
@@ -546,9 +552,18 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
 // NW waves side by side in rows, 32 rows each.  A stage is a step's K, then its V: rows of HD * ES bytes, whose 16-byte
 // pieces lie at their number ^ (row & 7), so that eight lanes that read one piece of eight rows meet eight different
 // bank groups.  Loads write LDS in lane order, so the lane that lands in a place fetches the piece that belongs there.
+#ifndef LK_WIDE_AIM
+#define LK_WIDE_AIM 4096
+#endif
+#ifndef LK_WIDE_FEW
+#define LK_WIDE_FEW 512
+#endif
+#ifndef LK_WIDE_LEAST
+#define LK_WIDE_LEAST 512
+#endif
 template <int HD, bool F32, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_wide_kernel(const LkPagedAttn a) {
-    constexpr int RT = 2, NT = F32 ? 2 : 4, STEP = NT * 16;
+    constexpr int RT = 2, NT = F32 || HD == 128 ? 2 : 4, STEP = NT * 16;
     using Wave = Rows<HD, F32, RT, NT, false>;
     constexpr int ND = Wave::ND, KS = F32 ? ND : Wave::KS, VW = Wave::VW, ES = Wave::ES;
     constexpr int RB = HD * ES, PIECES = RB / 16, PER = 64 / PIECES;   // rows that one load instruction covers
@@ -563,80 +578,84 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_wide_kernel(const LkPagedAtt
     const bool busy = rbase < h.R;  // wave-uniform; an idle wave loads with the others
     const uint32_t steps = (h.x1 - h.x0 + STEP - 1) / STEP;
 
-    // Page ids of the chunk's tiles, 64 at a time, one a lane; `ahead` are the next 64.
+    // Where the chunk's tiles lie, 64 at a time, one a lane (byte of the first row), and which are no holes; `ahead`:
+    // page ids of the next 64.
     auto ids_of = [&](uint32_t block) -> uint32_t {
         uint32_t pos;
         const uint64_t y = (uint64_t)h.x0 + ((uint64_t)block * 64 + lane) * 16;
         return y < h.x1 ? tile_page<false>(a, h, (uint32_t)y, pos) : LK_NO_PAGE;
     };
-    uint32_t ids = ids_of(0), ahead = ids_of(1), block = 0;
+    uint32_t at_lo, at_hi, block = 0;
+    uint64_t there;
+    auto place = [&](uint32_t id) {
+        const uint64_t at = tile_base(a, h, id, h.x0 + (block * 64 + lane) * 16, HD) * ES;
+        at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
+        there = __ballot(id < a.p.n_pages);
+    };
+    place(ids_of(0));
+    uint32_t ahead = ids_of(1);
     typedef __attribute__((address_space(3))) uint32_t* lptr;
     typedef __attribute__((address_space(1))) uint32_t* gptr;
+    // this lane's piece of an instruction's rows: the instruction's first row is a multiple of PER
+    const uint32_t in_op = lane / PIECES, my_piece = lane % PIECES;
     auto issue = [&](uint32_t n, char* stage) {
-        const uint32_t x = h.x0 + n * STEP;
 #pragma unroll
         for (int k = 0; k < OPS; k++) {
             const uint32_t q = w * OPS + k, row0 = q * PER % STEP;  // the K loads, then the V loads
-            const uint32_t tile = (n * STEP + row0) / 16;
-            const uint32_t id = __builtin_amdgcn_readlane(ids, tile & 63);
-            const uint32_t row = row0 + lane / PIECES, piece = (lane % PIECES) ^ (row & 7);
-            const uint64_t at = tile_base(a, h, id, x + (row0 & ~15u), HD) * ES + (row & 15) * RB + piece * 16;
+            const uint32_t tile = (n * NT + row0 / 16) & 63;
+            const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, tile) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, tile);
             const char* from = (const char*)(q * PER >= STEP ? a.p.v : a.p.k) + at;
-            __builtin_amdgcn_global_load_lds((gptr)from, (lptr)(stage + q * 1024), 16, 0, 0);
+            const uint32_t mine = ((row0 & 15) + in_op) * RB + ((my_piece ^ ((row0 + in_op) & 7)) * 16);
+            __builtin_amdgcn_global_load_lds((gptr)(from + mine), (lptr)(stage + q * 1024), 16, 0, 0);
         }
     };
-    // a step's ids before its issue: the next block of 64 begins every 64 / NT steps
+    // before a step's issue: the next 64 tiles begin every 64 / NT steps
     auto turn_page = [&](uint32_t n) {
         if (n * NT / 64 != block) {
             block++;
-            ids = ahead;
+            place(ahead);
             ahead = ids_of(block + 1);
         }
     };
-    // whether a step has something to hide, and which positions are there, is kept for the RING - 1 steps till its use
-    auto look = [&](uint32_t n, uint64_t& live) -> bool {
-        const uint32_t x = h.x0 + n * STEP;
-        live = 0;
-        bool masked = x + STEP > h.sq.ctx;
+    auto look = [&](uint32_t n) -> uint32_t { return (uint32_t)(there >> (n * NT & 63)) & ((1u << NT) - 1); };
+    // the positions of a step that a row may see; tiles: which are no holes
+    auto live_of = [&](uint32_t x, uint32_t tiles) -> uint64_t {
+        uint64_t b = 0;
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const uint32_t id = __builtin_amdgcn_readlane(ids, (n * NT + t) & 63);
-            masked |= id >= a.p.n_pages;
-            if (id < a.p.n_pages) live |= (low_bits((int64_t)h.sq.total - (x + 16 * t)) & 0xFFFF) << (16 * t);
-        }
-        return masked;
+        for (int t = 0; t < NT; t++) b |= tiles >> t & 1 ? 0xFFFFull << (16 * t) : 0;
+        return b & low_bits((int64_t)h.sq.total - x);
     };
     Wave r;
-    // of the steps under way: what is there, and whether something is to be hidden
-    uint64_t live[RING - 1];
-    bool masked[RING - 1];
+    uint32_t tiles[RING - 1];  // of the steps under way: which tiles are no holes
 #pragma unroll
     for (int n = 0; n < RING - 1; n++) {
-        masked[n] = false, live[n] = 0;
+        tiles[n] = 0;
         if ((uint32_t)n < steps) {
-            masked[n] = look(n, live[n]);
+            tiles[n] = look(n);
             issue(n, ring[n]);
         }
     }
     r.init(a, h, rbase);
-    auto scores = [&](const char* stage) {
+    // where the lane reads a stage: K piece 4 ks + j of row c16, V's dims of row 4 j + i; a tile further 16 rows on
+    uint32_t k_at[KS], v_at[4][VW > 4 ? 2 : 1];
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const uint32_t row = 16 * t + r.c16;
+    for (int ks = 0; ks < KS; ks++) k_at[ks] = r.c16 * RB + ((4 * ks + r.j) ^ (r.c16 & 7)) * 16;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) r.scores(t, ks, *(const u4*)(stage + row * RB + ((4 * ks + r.j) ^ (row & 7)) * 16));
-        }
-    };
+    for (int i = 0; i < 4; i++) {
+        const uint32_t row = 4 * r.j + i;
+        if constexpr (VW == 2) v_at[i][0] = HALF + row * RB + ((r.c16 / 2) ^ (row & 7)) * 16 + (r.c16 & 1) * 8;
+        else
+#pragma unroll
+            for (int d = 0; d < VW; d += 4) v_at[i][d / 4] = HALF + row * RB + ((4 * d + r.c16) ^ (row & 7)) * 16;
+    }
     auto value = [&](const char* stage, int t, int i, uint32_t (&v)[VW]) {
-        const uint32_t row = 16 * t + 4 * r.j + i;
-        const char* at = stage + HALF + row * RB;
         if constexpr (VW == 2) {
-            const u2 y = *(const u2*)(at + ((r.c16 / 2) ^ (row & 7)) * 16 + (r.c16 & 1) * 8);
+            const u2 y = *(const u2*)(stage + v_at[i][0] + t * 16 * RB);
             v[0] = y[0], v[1] = y[1];
         } else {
 #pragma unroll
             for (int d = 0; d < VW; d += 4) {
-                const u4 y = *(const u4*)(at + ((d * 4 + r.c16) ^ (row & 7)) * 16);
+                const u4 y = *(const u4*)(stage + v_at[i][d / 4] + t * 16 * RB);
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[d + e] = y[e];
             }
@@ -647,21 +666,26 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_wide_kernel(const LkPagedAtt
         // step n has landed for every wave, and every wave is done with the stage that is filled next
         if (RING > 2 && n + RING - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * OPS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const bool mk = masked[0];
-        const uint64_t lv = live[0];
+        const uint32_t tl = tiles[0];
 #pragma unroll
-        for (int k = 0; k + 1 < RING - 1; k++) masked[k] = masked[k + 1], live[k] = live[k + 1];
+        for (int k = 0; k + 1 < RING - 1; k++) tiles[k] = tiles[k + 1];
         if (n + RING - 1 < steps) {
             turn_page(n + RING - 1);
-            masked[RING - 2] = look(n + RING - 1, live[RING - 2]);
+            tiles[RING - 2] = look(n + RING - 1);
             issue(n + RING - 1, ring[slot ? slot - 1 : RING - 1]);
         }
         const char* stage = ring[slot];
         slot = slot + 1 < RING ? slot + 1 : 0;
         if (!busy) continue;
         const uint32_t x = h.x0 + n * STEP;
-        scores(stage);
+        const bool mk = tl != (1u << NT) - 1 || x + STEP > h.sq.ctx;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) r.scores(t, ks, *(const u4*)(stage + k_at[ks] + t * 16 * RB));
+        uint64_t lv = 0;
         if (mk) {
+            lv = live_of(x, tl);
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, lv, rt));
         }
@@ -762,7 +786,13 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
     const uint64_t base = (uint64_t)n * n_kv * p.n_rg;
     const uint32_t step = p.narrow ? (f32 || hd == 128 ? 32 : 64) * 4 : 64;  // narrow: every wave has a step
     const uint64_t steps = (positions + step - 1) / step;
-    uint64_t c = (1024 + base - 1) / base;
+    const uint64_t aim = p.narrow ? 1024 : LK_WIDE_AIM, few = LK_WIDE_FEW, least = LK_WIDE_LEAST;
+    uint64_t c = (aim + base - 1) / base;
+    if (!p.narrow && c > 1) {  // long chunks, unless there are few
+        const uint64_t by_len = (positions + least - 1) / least, by_fill = (few + base - 1) / base;
+        const uint64_t most = by_len > by_fill ? by_len : by_fill;
+        c = c < most ? c : most;
+    }
     c = c > kMaxChunks ? kMaxChunks : c;
     c = c > steps ? steps : c;
     if (c < 1) c = 1;
