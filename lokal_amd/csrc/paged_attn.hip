@@ -43,10 +43,12 @@ namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __fp16 p2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
+#define LK_INLINE __attribute__((always_inline))  // lambdas too: what they capture stays in registers
 constexpr float kLag = 8.f;  // log2: how far a score may pass the running maximum
 constexpr uint32_t kMaxChunks = 64;
 
@@ -88,29 +90,33 @@ __device__ __forceinline__ uint32_t chunks_of(uint32_t total, uint32_t chunk) {
     return c ? c : 1;
 }
 
-// A workgroup's share: one chunk of a (sequence, kv head)'s positions and one group of its rows.  Row groups of one
-// chunk read the same K and V: they run on one XCD (workgroups go round the 8), one after the other.
+// A workgroup's share: some of the positions of a (sequence, kv head), and one group of its rows.
 struct Share {
-    uint32_t s, kvh, pair, chunk, row0, R, x0, x1, nch;
+    uint32_t s, kvh, row0, R, x0, x1;
     Seq sq;
     bool live;
+    bool whole;   // all of the rows' positions: the output can be written
+    size_t part;  // else: where the first row's part goes
 };
+// The narrow kernel's: one chunk.  Row groups of one chunk read the same K and V: they run on one XCD (workgroups go
+// round the 8), one after the other.
 template <bool SPARSE>
 __device__ __forceinline__ Share share_of(const LkPagedAttn& a, uint32_t rows) {
     Share h{};
     const uint32_t xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
     const uint32_t rg = turn % a.n_rg, item = turn / a.n_rg * 8 + xcd;
     if (item >= a.n * a.p.n_kv * a.n_chunks) return h;
-    h.chunk = item % a.n_chunks;
-    h.pair = item / a.n_chunks;
-    h.kvh = h.pair % a.p.n_kv;
-    h.s = h.pair / a.p.n_kv;
+    const uint32_t pair = item / a.n_chunks;
+    const uint32_t chunk = (item % a.n_chunks + pair) % a.n_chunks;  // short sequences lack the same chunks: not the same XCDs'
+    h.kvh = pair % a.p.n_kv;
+    h.s = pair / a.p.n_kv;
     h.sq = seq_of<SPARSE>(a, h.s);
     h.R = h.sq.rows * a.G;
     h.row0 = rg * rows;
-    h.x0 = h.chunk * a.chunk;
-    h.live = h.sq.live && h.row0 < h.R && (h.x0 < h.sq.total || h.chunk == 0);
-    h.nch = chunks_of(h.sq.total, a.chunk);
+    h.x0 = chunk * a.chunk;
+    h.live = h.sq.live && h.row0 < h.R && (h.x0 < h.sq.total || chunk == 0);
+    h.whole = chunks_of(h.sq.total, a.chunk) == 1;
+    h.part = ((size_t)pair * a.n_chunks + chunk) * a.rows_pad + h.row0;
     h.x1 = h.x0 + a.chunk < h.sq.total ? h.x0 + a.chunk : h.sq.total;
     return h;
 }
@@ -134,27 +140,32 @@ __device__ __forceinline__ uint64_t tile_base(const LkPagedAttn& a, const Share&
            h.kvh * a.p.head_stride;
 }
 
-// Dim d (0..HD / 16 - 1) of lane column c16 in the second product.
-template <int HD, bool F32>
+// Dim d (0..HD / 16 - 1) of lane column c16 in the second product.  TR: V comes through LDS's transposing reads.
+template <int HD, bool F32, bool TR>
 __device__ __forceinline__ constexpr uint32_t dim_of(uint32_t c16, int d) {
-    return F32 ? (d / 4) * 64 + 4 * c16 + d % 4 : HD / 16 * c16 + d;
+    return TR ? 16 * d + c16 : F32 ? (d / 4) * 64 + 4 * c16 + d % 4 : HD / 16 * c16 + d;
 }
 
 // A wave's RT tiles of 16 rows: their queries, running maxima and sums, and O.
-template <int HD, bool F32, int RT, int NT, bool SPARSE>
+template <int HD, bool F32, int RT, int NT, bool SPARSE, bool TR>
 struct Rows {
-    static constexpr int ND = HD / 16, KS = HD / 32, ES = F32 ? 4 : 2;
+    static constexpr int ND = HD / 16, KS = F32 ? ND : HD / 32, ES = F32 ? 4 : 2;
     static constexpr int VW = ND * ES / 4;  // words of a lane's dims of one V row
     h8 qh[F32 ? 1 : RT][F32 ? 1 : KS], ql[F32 ? 1 : RT][F32 ? 1 : KS];
     f4 qf[F32 ? RT : 1][F32 ? ND : 1];
-    float fac[RT], m[RT], l[RT];
+    float m[RT];     // log2: what row c16's weights are relative to; -inf before its first score
+    float l[F32 ? RT : 1];  // lane's part of row c16's sum
+    f4 lr[F32 ? 1 : RT];    // sums of rows 4 j + i, by a product with ones: the matrix cores have time, the adders not
     uint32_t tok[RT];
     f4 o[RT][ND];
-    f4 sc[RT][NT];
+    int up[RT];      // q was taken times 2^up: 0 for rows whose largest value needs no scaling
     uint32_t j, c16;
+    using Scores = f4[RT][NT];
 
-    __device__ __forceinline__ void init(const LkPagedAttn& a, const Share& h, uint32_t rbase) {
+    // Whether some row's up is not 0.
+    __device__ __forceinline__ bool init(const LkPagedAttn& a, const Share& h, uint32_t rbase) {
         j = (threadIdx.x & 63) >> 4, c16 = threadIdx.x & 15;
+        bool scaled = false;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const uint32_t row = rbase + rt * 16 + c16;
@@ -163,11 +174,11 @@ struct Rows {
             const uint32_t g = live ? row - tok[rt] * a.G : 0;
             const float* q = a.q + (((size_t)h.s * a.tokens + tok[rt]) * a.n_heads + h.kvh * a.G + g) * HD;
             m[rt] = -INFINITY;
-            l[rt] = 0.f;
+            if constexpr (F32) l[rt] = 0.f, up[rt] = 0;
+            else lr[rt] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < ND; d++) o[rt][d] = f4{0.f, 0.f, 0.f, 0.f};
             if constexpr (F32) {
-                fac[rt] = 1.f;
 #pragma unroll
                 for (int b = 0; b < ND; b++) {  // dims 16 b + 4 j + e
                     const f4 x = *(const f4*)(q + 16 * b + 4 * j);
@@ -175,6 +186,7 @@ struct Rows {
                 }
             } else {
                 float x[KS][8], top = 0.f;
+                int by = 0;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {  // dims 32 ks + 8 j + e
                     const f4 u = *(const f4*)(q + 32 * ks + 8 * j), v = *(const f4*)(q + 32 * ks + 8 * j + 4);
@@ -186,42 +198,65 @@ struct Rows {
                 }
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
-                int up = 0;
-                if (top > 0.f && top < INFINITY) {
-                    up = 13 + 127 - (int)((__float_as_uint(top) >> 23) & 255);
-                    up = up > 100 ? 100 : up;  // subnormal rows
+                // Rows whose largest value is in [1/4, 2^14) are split as they are: the second part, down to f16's
+                // 2^-24, is off by 2^-23 of it at most.  Others are brought to 2^13..2^14 first.
+                if (top > 0.f && top < INFINITY && (top < 0.25f || top >= 16384.f)) {
+                    by = 13 + 127 - (int)((__float_as_uint(top) >> 23) & 255);
+                    by = by > 100 ? 100 : by;  // subnormal rows
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[ks][e] = ldexpf(x[ks][e], by);
                 }
-                fac[rt] = ldexpf(1.f, -up);
+                up[rt] = by;
+                scaled |= __any(by != 0);
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float y = ldexpf(x[ks][e], up);
-                        const _Float16 hi = (_Float16)y;
+                        const _Float16 hi = (_Float16)x[ks][e];
                         qh[rt][ks][e] = hi;
-                        ql[rt][ks][e] = (_Float16)(y - (float)hi);
+                        ql[rt][ks][e] = (_Float16)(x[ks][e] - (float)hi);
                     }
             }
         }
+        return scaled;
     }
 
-    // K operand: f16 the lane's 8 dims 32 ks + 8 j of position c16, f32 its 4 dims 16 b + 4 j
-    __device__ __forceinline__ void scores(int t, int ks, u4 k) {
-        if constexpr (F32) {
-            const f4 kk = __builtin_bit_cast(f4, k);
+    // Scores relative to m: the products start at -m.  k: f16 the lane's 8 dims 32 ks + 8 j of position c16, f32 its 4
+    // dims 16 ks + 4 j.  Products that follow each other belong to different sums.
+    __device__ __forceinline__ void scores(const u4 (&k)[NT][KS], Scores& sc) const {
+        f4 c[RT];
 #pragma unroll
-            for (int e = 0; e < 4; e++)
+        for (int rt = 0; rt < RT; rt++) {
+            float z = m[rt] == -INFINITY ? 0.f : -m[rt];
+            if constexpr (!F32) z = ldexpf(z, up[rt]);
+            c[rt] = f4{z, z, z, z};
+        }
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-                    sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], qf[rt][ks][e], ks == 0 && e == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sc[rt][t], 0, 0, 0);
-        } else {
-            const h8 kk = __builtin_bit_cast(h8, k);
+        for (int ks = 0; ks < KS; ks++) {
+            if constexpr (F32) {
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++)
-                sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[rt][ks], ks == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sc[rt][t], 0, 0, 0);
+                for (int e = 0; e < 4; e++)
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++)
-                sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[rt][ks], sc[rt][t], 0, 0, 0);
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+                            sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, k[t][ks])[e], qf[rt][ks][e],
+                                                                             ks == 0 && e == 0 ? c[rt] : sc[rt][t], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+                        sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, k[t][ks]), qh[rt][ks],
+                                                                           ks == 0 ? c[rt] : sc[rt][t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+                        sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, k[t][ks]), ql[rt][ks], sc[rt][t], 0, 0, 0);
+            }
         }
     }
 
@@ -247,7 +282,7 @@ struct Rows {
         }
         return live & (low_bits(-off) | draft);
     }
-    __device__ __forceinline__ void hide(int rt, uint64_t see) {
+    __device__ __forceinline__ void hide(int rt, uint64_t see, Scores& sc) const {
         const uint32_t b[2] = {(uint32_t)see >> (4 * j), (uint32_t)(see >> 32) >> (4 * j)};
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -255,42 +290,53 @@ struct Rows {
             for (int i = 0; i < 4; i++) sc[rt][t][i] = b[t / 2] >> (16 * (t & 1) + i) & 1 ? sc[rt][t][i] : -INFINITY;
     }
 
-    // Scores become weights; running maximum and sum.
-    __device__ __forceinline__ void weigh(int rt) {
-        float top = -INFINITY;
+    // Before scores become weights: m moves up where one passes it by kLag.
+    __device__ __forceinline__ void move(Scores& sc, bool scaled) {
+        float top[RT];
+        bool far = false;
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int rt = 0; rt < RT; rt++) {
+            if (!F32 && scaled) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) top = fmaxf(top, sc[rt][t][i]);
-        top *= fac[rt];  // a power of two
-        if (__any(top > m[rt] + kLag)) {
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m[rt], top);
-            const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - mn);
-            m[rt] = mn;
-            l[rt] *= f;
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[rt][t][i] = ldexpf(sc[rt][t][i], -up[rt]);
+            }
+            top[rt] = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) top[rt] = fmaxf(top[rt], sc[rt][t][i]);
+            far |= top[rt] > (m[rt] == -INFINITY ? -INFINITY : kLag);
+        }
+        if (!__any(far)) return;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const bool first = m[rt] == -INFINITY;
+            float x = top[rt];
+            x = fmaxf(x, __shfl_xor(x, 16, 64));
+            x = fmaxf(x, __shfl_xor(x, 32, 64));
+            const float by = first ? (x == -INFINITY ? 0.f : x) : fmaxf(x, 0.f);  // how far m goes up
+            const float f = first ? 1.f : __builtin_amdgcn_exp2f(-by);
+            m[rt] = first ? x : m[rt] + by;
+#pragma unroll
+            for (int t = 0; t < NT; t++) sc[rt][t] -= by;
+            if constexpr (F32) l[rt] *= f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float fi = __shfl(f, (int)(4 * j + i), 64);  // O's rows are 4 j + i
+                if constexpr (!F32) lr[rt][i] *= fi;
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[rt][d][i] *= fi;
             }
         }
-        const float ms = m[rt] == -INFINITY ? 0.f : m[rt];  // no score yet: weights of 0
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(sc[rt][t][i], fac[rt], -ms));
-                sc[rt][t][i] = p;
-                l[rt] += p;
-            }
     }
 
-    // v[i]: the lane's dims of position 4 j + i.  f16: two tiles 2 g, 2 g + 1 at once (v, w)
-    __device__ __forceinline__ void add16(int g, const uint32_t (&v)[4][VW], const uint32_t (&w)[4][VW]) {
-        h8 ph[RT], pl[RT];
+    // f16: tiles 2 g and 2 g + 1.  vb[d]: column tile d of their V, positions 4 j + i of the one, then of the other
+    __device__ __forceinline__ void add16(const Scores& sc, int g, const h8 (&vb)[ND]) {
+        h8 ph[RT], pl[RT], ones;
+#pragma unroll
+        for (int e = 0; e < 8; e++) ones[e] = (_Float16)1.f;
         float minus = -1.f;  // a register: p - hi is then one mixed product, hi not widened first
         asm("" : "+s"(minus));
 #pragma unroll
@@ -298,7 +344,8 @@ struct Rows {
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {  // truncated to f16; what that leaves fits f16's 11 bits but for two
-                const float p0 = sc[rt][2 * g + e / 2][2 * (e & 1)], p1 = sc[rt][2 * g + e / 2][2 * (e & 1) + 1];
+                const float p0 = __builtin_amdgcn_exp2f(sc[rt][2 * g + e / 2][2 * (e & 1)]),
+                            p1 = __builtin_amdgcn_exp2f(sc[rt][2 * g + e / 2][2 * (e & 1) + 1]);
                 const p2 u = __builtin_amdgcn_cvt_pkrtz(p0, p1);
                 hi[e] = __builtin_bit_cast(uint32_t, u);
                 lo[e] = __builtin_bit_cast(
@@ -308,50 +355,55 @@ struct Rows {
             pl[rt] = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
         }
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const uint32_t pick = (d & 1) ? 0x07060302u : 0x05040100u;  // halves d of two positions
-            const h8 vb = __builtin_bit_cast(
-                h8, u4{__builtin_amdgcn_perm(v[1][d / 2], v[0][d / 2], pick), __builtin_amdgcn_perm(v[3][d / 2], v[2][d / 2], pick),
-                       __builtin_amdgcn_perm(w[1][d / 2], w[0][d / 2], pick), __builtin_amdgcn_perm(w[3][d / 2], w[2][d / 2], pick)});
+        for (int part = 0; part < 2; part++) {
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[rt], vb, o[rt][d], 0, 0, 0);
+            for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[rt], vb, o[rt][d], 0, 0, 0);
+                for (int rt = 0; rt < RT; rt++)
+                    o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part ? pl[rt] : ph[rt], vb[d], o[rt][d], 0, 0, 0);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) lr[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part ? pl[rt] : ph[rt], ones, lr[rt], 0, 0, 0);
         }
     }
-    __device__ __forceinline__ void add32(int t, int i, const uint32_t (&v)[VW]) {
+    __device__ __forceinline__ void add32(const Scores& sc, int t, int i, const uint32_t (&v)[VW]) {
+        float p[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            p[rt] = __builtin_amdgcn_exp2f(sc[rt][t][i]);
+            l[rt] += p[rt];
+        }
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
-                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[rt][t][i], __uint_as_float(v[d % VW]), o[rt][d], 0, 0, 0);
+                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[rt], __uint_as_float(v[d % VW]), o[rt][d], 0, 0, 0);
     }
 
-    // In a masked step: V of positions that no row sees becomes zero, and what is not finite too; the result says
-    // whether there was any.
+    // A word of V in a masked step: what is not finite becomes zero, and odd says so.
+    static __device__ __forceinline__ uint32_t clean_word(uint32_t y, uint32_t& odd) {
+        if constexpr (F32) {
+            const bool bad = not_finite(__uint_as_float(y));
+            odd |= bad;
+            return bad ? 0 : y;
+        } else {
+            const uint32_t bad = halves_not_finite(y);
+            odd |= bad;
+            return y & ~((bad >> 15) * 0xFFFFu);
+        }
+    }
+    // V of position 4 j + i of tile t: zero where no row sees it.
     __device__ __forceinline__ uint32_t clean(int t, int i, uint64_t live, uint32_t (&v)[VW]) const {
         const bool see = live >> (16 * t + 4 * j + i) & 1;
         uint32_t odd = 0;
 #pragma unroll
         for (int d = 0; d < VW; d++) {
-            uint32_t y = see ? v[d] : 0;
-            if constexpr (!SPARSE) {
-                if constexpr (F32) {
-                    const bool bad = not_finite(__uint_as_float(y));
-                    odd |= bad;
-                    y = bad ? 0 : y;
-                } else {
-                    const uint32_t bad = halves_not_finite(y);
-                    odd |= bad;
-                    y &= ~((bad >> 15) * 0xFFFFu);
-                }
-            }
-            v[d] = y;
+            v[d] = see ? v[d] : 0;
+            if constexpr (!SPARSE) v[d] = clean_word(v[d], odd);
         }
         return odd;
     }
     // Rows that see a value that is not finite: NaN in its dim.  Rare, so short: a position at a time.
-    __device__ void poison(const LkPagedAttn& a, const Share& h, uint32_t x, uint64_t live) {
+    __device__ __forceinline__ void poison(const LkPagedAttn& a, const Share& h, uint32_t x, uint64_t live) {
         for (uint32_t p = 0; p < NT * 16; p++) {
             if (!(live >> p & 1)) continue;  // uniform
             uint32_t pos;
@@ -360,7 +412,7 @@ struct Rows {
             uint32_t bad = 0;
 #pragma unroll
             for (int d = 0; d < ND; d++) {
-                const uint64_t e = at + dim_of<HD, F32>(c16, d);
+                const uint64_t e = at + dim_of<HD, F32, TR>(c16, d);
                 bool b;
                 if constexpr (F32) b = not_finite(((const float*)a.p.v)[e]);
                 else b = (((const uint16_t*)a.p.v)[e] & 0x7C00) == 0x7C00;
@@ -380,32 +432,41 @@ struct Rows {
         }
     }
 
-    // row sums over the lanes that share a row
-    __device__ __forceinline__ void close() {
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            l[rt] += __shfl_xor(l[rt], 16, 64);
-            l[rt] += __shfl_xor(l[rt], 32, 64);
+    // Sum of row 4 j + i of tile rt, on its lanes.
+    __device__ __forceinline__ float sum_of(int rt, int i) const {
+        if constexpr (F32) {
+            float x = l[rt];
+            x += __shfl_xor(x, 16, 64);
+            x += __shfl_xor(x, 32, 64);
+            return __shfl(x, (int)(4 * j + i), 64);
+        } else {
+            return lr[rt][i];
         }
     }
+    __device__ __forceinline__ float max_of(int rt, int i) const { return __shfl(m[rt], (int)(4 * j + i), 64); }
     // Row lr of the workgroup: the output where the sequence has one chunk, else the chunk's (m, sum, O).
     __device__ __forceinline__ void put(const LkPagedAttn& a, const Share& h, uint32_t lr, float top, float sum, float (&y)[ND]) const {
         const uint32_t row = h.row0 + lr;
         if (row >= h.R) return;
         float* to;
-        if (h.nch == 1) {
+        if (h.whole) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: zeros
 #pragma unroll
             for (int d = 0; d < ND; d++) y[d] *= inv;
             const uint32_t t = row / a.G;
             to = a.out + (((size_t)h.s * a.tokens + t) * a.n_heads + h.kvh * a.G + row - t * a.G) * HD;
         } else {
-            const size_t at = ((size_t)h.pair * a.n_chunks + h.chunk) * a.rows_pad + row;
+            const size_t at = h.part + lr;
             if (c16 == 0) *(float2*)(a.part_ml + 2 * at) = float2{top, sum};
             to = a.part_o + at * HD;
         }
+        if constexpr (TR) {
 #pragma unroll
-        for (int d = 0; d < ND; d += 4) *(f4*)(to + dim_of<HD, F32>(c16, d)) = f4{y[d], y[d + 1], y[d + 2], y[d + 3]};
+            for (int d = 0; d < ND; d++) to[dim_of<HD, F32, TR>(c16, d)] = y[d];
+        } else {
+#pragma unroll
+            for (int d = 0; d < ND; d += 4) *(f4*)(to + dim_of<HD, F32, TR>(c16, d)) = f4{y[d], y[d + 1], y[d + 2], y[d + 3]};
+        }
     }
 };
 
@@ -414,18 +475,19 @@ struct Rows {
 template <int HD, bool F32, int RT, bool SPARSE>
 __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) {
     constexpr int NT = F32 || HD == 128 ? 2 : 4, W = 4, ROWS = RT * 16, STEP = NT * 16;
-    using Wave = Rows<HD, F32, RT, NT, SPARSE>;
-    constexpr int ND = Wave::ND, KS = F32 ? ND : Wave::KS, VW = Wave::VW, ES = Wave::ES;
+    using Wave = Rows<HD, F32, RT, NT, SPARSE, false>;
+    constexpr int ND = Wave::ND, KS = Wave::KS, VW = Wave::VW, ES = Wave::ES;
     __shared__ float s_m[W][ROWS], s_l[W][ROWS];
     __shared__ __align__(16) float s_o[ROWS][HD + 4];
     const Share h = share_of<SPARSE>(a, ROWS);
     if (!h.live) return;  // uniform
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Wave r;
+    bool scaled;
     u4 kr[2][NT][KS];
     uint32_t vr[2][NT][4][VW];
     // a step's tiles: loads go out for all of its K and V
-    auto fetch = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t& live, bool& masked) {
+    auto fetch = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t& live, bool& masked) LK_INLINE {
         const uint32_t j = (threadIdx.x & 63) >> 4, c16 = threadIdx.x & 15;
         live = 0;
         masked = false;
@@ -453,7 +515,7 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
                 const char* row = vb[t] + (4 * j + i) * HD * ES;
 #pragma unroll
                 for (int d = 0; d < ND; d += 16 / ES < ND ? 16 / ES : ND) {
-                    const char* at = row + dim_of<HD, F32>(c16, d) * ES;
+                    const char* at = row + dim_of<HD, F32, false>(c16, d) * ES;
                     if constexpr (VW == 2) {
                         const u2 y = *(const u2*)at;
                         v[t][i][0] = y[0], v[t][i][1] = y[1];
@@ -465,14 +527,12 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
                 }
             }
     };
-    auto use = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t live, bool masked) {
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) r.scores(t, ks, k[t][ks]);
+    auto use = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t live, bool masked) LK_INLINE {
+        f4 sc[RT][NT];
+        r.scores(k, sc);
         if (__builtin_amdgcn_readfirstlane(masked)) {
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt));
+            for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt), sc);
             uint32_t odd = 0;
 #pragma unroll
             for (int t = 0; t < NT; t++)
@@ -480,23 +540,34 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
                 for (int i = 0; i < 4; i++) odd |= r.clean(t, i, live, v[t][i]);
             if (__any(odd)) r.poison(a, h, x, live);
         }
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) r.weigh(rt);
+        r.move(sc, scaled);
         if constexpr (F32) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) r.add32(t, i, v[t][i]);
+                for (int i = 0; i < 4; i++) r.add32(sc, t, i, v[t][i]);
         } else {
 #pragma unroll
-            for (int g = 0; g < NT / 2; g++) r.add16(g, v[2 * g], v[2 * g + 1]);
+            for (int g = 0; g < NT / 2; g++) {
+                h8 vb[ND];
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const uint32_t pick = (d & 1) ? 0x07060302u : 0x05040100u;  // halves d of two positions
+                    u4 y;
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        y[e] = __builtin_amdgcn_perm(v[2 * g + e / 2][2 * (e & 1) + 1][d / 2], v[2 * g + e / 2][2 * (e & 1)][d / 2], pick);
+                    vb[d] = __builtin_bit_cast(h8, y);
+                }
+                r.add16(sc, g, vb);
+            }
         }
     };
     uint32_t x = h.x0 + w * STEP;
     uint64_t live[2];
     bool masked[2];
     if (x < h.x1) fetch(x, kr[0], vr[0], live[0], masked[0]);
-    r.init(a, h, h.row0);
+    scaled = r.init(a, h, h.row0);
     while (x < h.x1) {
         uint32_t nx = x + W * STEP;
         if (nx < h.x1) fetch(nx, kr[1], vr[1], live[1], masked[1]);
@@ -509,10 +580,13 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
         x = nx;
     }
     // ---- the waves join: m and sum per row, then O one wave after the other
-    r.close();
 #pragma unroll
     for (int rt = 0; rt < RT; rt++)
-        if (r.j == 0) s_m[w][rt * 16 + r.c16] = r.m[rt], s_l[w][rt * 16 + r.c16] = r.l[rt];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float mi = r.max_of(rt, i), li = r.sum_of(rt, i);
+            if (r.c16 == 0) s_m[w][rt * 16 + 4 * r.j + i] = mi, s_l[w][rt * 16 + 4 * r.j + i] = li;
+        }
     __syncthreads();
     for (uint32_t turn = 0; turn < W; turn++) {
         if (w == turn) {
@@ -533,7 +607,7 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
                     for (int d = 0; d < ND; d++) y[d] = r.o[rt][d][i] * f;
 #pragma unroll
                     for (int d = 0; d < ND; d += 4) {
-                        f4* acc = (f4*)&s_o[lr][dim_of<HD, F32>(r.c16, d)];
+                        f4* acc = (f4*)&s_o[lr][dim_of<HD, F32, false>(r.c16, d)];
                         f4 z = f4{y[d], y[d + 1], y[d + 2], y[d + 3]};
                         if (turn > 0) z += *acc;
                         if (turn < W - 1) *acc = z;
@@ -549,209 +623,372 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
 
 // ------------------------------------------------------------------ wide
 
-// NW waves side by side in rows, 32 rows each.  A stage is a step's K, then its V: rows of HD * ES bytes, whose 16-byte
-// pieces lie at their number ^ (row & 7), so that eight lanes that read one piece of eight rows meet eight different
-// bank groups.  Loads write LDS in lane order, so the lane that lands in a place fetches the piece that belongs there.
-#ifndef LK_WIDE_AIM
-#define LK_WIDE_AIM 4096
+// Work of the wide kernel is counted in steps of an item: a (sequence, kv head, group of ROWS rows), all items one
+// after the other, row groups of a kv head together.  How many there are is known on the device only (contexts and
+// drafts differ), so a fixed number of workgroups, as many as the card holds at once, takes equal runs of steps; a run
+// may end one item and begin others.  Fixed chunks of the table's capacity left half the card idle behind the last
+// of 565 live workgroups on 512 places (8 x 64 tokens over up to 32768 positions: 214 us).
+struct Plan {
+    uint64_t total;
+    uint32_t run;  // steps of a workgroup
+};
+// Steps of one item of a sequence, and its items.
+__device__ __forceinline__ uint32_t item_steps(const Seq& q, uint32_t step) { return (q.total + step - 1) / step; }
+__device__ __forceinline__ uint32_t row_groups(const LkPagedAttn& a, const Seq& q, uint32_t rows) {
+    return q.live ? (q.rows * a.G + rows - 1) / rows : 0;
+}
+#ifndef LK_LEAST
+#define LK_LEAST 2
 #endif
-#ifndef LK_WIDE_FEW
-#define LK_WIDE_FEW 512
-#endif
-#ifndef LK_WIDE_LEAST
-#define LK_WIDE_LEAST 512
-#endif
-template <int HD, bool F32, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void paged_wide_kernel(const LkPagedAttn a) {
-    constexpr int RT = 2, NT = F32 || HD == 128 ? 2 : 4, STEP = NT * 16;
-    using Wave = Rows<HD, F32, RT, NT, false>;
-    constexpr int ND = Wave::ND, KS = F32 ? ND : Wave::KS, VW = Wave::VW, ES = Wave::ES;
-    constexpr int RB = HD * ES, PIECES = RB / 16, PER = 64 / PIECES;   // rows that one load instruction covers
-    constexpr int HALF = STEP * RB, STAGE = 2 * HALF, OPS = STAGE / 1024 / NW;
-    constexpr int RING = STAGE <= 16384 ? 3 : 2;
-    static_assert(OPS >= 1 && STAGE % (1024 * NW) == 0 && 16 % PER == 0, "whole load instructions, each within a tile");
-    __shared__ __align__(1024) char ring[RING][STAGE];
-    const Share h = share_of<false>(a, NW * 32);
-    if (!h.live) return;  // uniform
-    const uint32_t lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t rbase = h.row0 + w * 32;
-    const bool busy = rbase < h.R;  // wave-uniform; an idle wave loads with the others
-    const uint32_t steps = (h.x1 - h.x0 + STEP - 1) / STEP;
+constexpr uint32_t kLeast = LK_LEAST;  // steps of a run at least
 
-    // Where the chunk's tiles lie, 64 at a time, one a lane (byte of the first row), and which are no holes; `ahead`:
-    // page ids of the next 64.
-    auto ids_of = [&](uint32_t block) -> uint32_t {
-        uint32_t pos;
-        const uint64_t y = (uint64_t)h.x0 + ((uint64_t)block * 64 + lane) * 16;
-        return y < h.x1 ? tile_page<false>(a, h, (uint32_t)y, pos) : LK_NO_PAGE;
+// All workgroups count all sequences; `start`: where this one's run begins.  Sequences are read twice (total, then
+// the place) unless one round of the threads holds them.  Workgroup 0 leaves the sequences' places for the fold.
+template <int NW>
+__device__ __forceinline__ Plan plan_runs(const LkPagedAttn& a, uint32_t wg, uint32_t step, uint32_t rows, uint32_t& seq,
+                                          uint64_t& in_seq) {
+    constexpr uint32_t T = NW * 64;
+    __shared__ uint64_t s_sum[NW];
+    __shared__ uint32_t s_long[NW];
+    __shared__ uint64_t s_at;
+    __shared__ uint32_t s_seq;
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    Plan p{};
+    uint32_t longest = 0;
+    auto count = [&](uint32_t s, uint32_t& steps) LK_INLINE -> uint64_t {
+        steps = 0;
+        if (s >= a.n) return 0;
+        const Seq q = seq_of<false>(a, s);
+        const uint32_t g = row_groups(a, q, rows);
+        steps = g ? item_steps(q, step) : 0;
+        return (uint64_t)g * a.p.n_kv * steps;
     };
-    uint32_t at_lo, at_hi, block = 0;
-    uint64_t there;
-    auto place = [&](uint32_t id) {
-        const uint64_t at = tile_base(a, h, id, h.x0 + (block * 64 + lane) * 16, HD) * ES;
-        at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
-        there = __ballot(id < a.p.n_pages);
-    };
-    place(ids_of(0));
-    uint32_t ahead = ids_of(1);
-    typedef __attribute__((address_space(3))) uint32_t* lptr;
-    typedef __attribute__((address_space(1))) uint32_t* gptr;
-    // this lane's piece of an instruction's rows: the instruction's first row is a multiple of PER
-    const uint32_t in_op = lane / PIECES, my_piece = lane % PIECES;
-    auto issue = [&](uint32_t n, char* stage) {
+    // exclusive sum over the block, and the sum
+    auto scan = [&](uint64_t v, uint64_t& all) LK_INLINE -> uint64_t {
+        uint64_t x = v;
 #pragma unroll
-        for (int k = 0; k < OPS; k++) {
-            const uint32_t q = w * OPS + k, row0 = q * PER % STEP;  // the K loads, then the V loads
-            const uint32_t tile = (n * NT + row0 / 16) & 63;
-            const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, tile) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, tile);
-            const char* from = (const char*)(q * PER >= STEP ? a.p.v : a.p.k) + at;
-            const uint32_t mine = ((row0 & 15) + in_op) * RB + ((my_piece ^ ((row0 + in_op) & 7)) * 16);
-            __builtin_amdgcn_global_load_lds((gptr)(from + mine), (lptr)(stage + q * 1024), 16, 0, 0);
+        for (int d = 1; d < 64; d *= 2) {
+            const uint64_t y = __shfl_up(x, d, 64);
+            if ((int)lane >= d) x += y;
         }
-    };
-    // before a step's issue: the next 64 tiles begin every 64 / NT steps
-    auto turn_page = [&](uint32_t n) {
-        if (n * NT / 64 != block) {
-            block++;
-            place(ahead);
-            ahead = ids_of(block + 1);
+        __syncthreads();
+        if (lane == 63) s_sum[w] = x;
+        __syncthreads();
+        uint64_t before = 0;
+        all = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < NW; k++) {
+            if (k < w) before += s_sum[k];
+            all += s_sum[k];
         }
+        return before + x - v;
     };
-    auto look = [&](uint32_t n) -> uint32_t { return (uint32_t)(there >> (n * NT & 63)) & ((1u << NT) - 1); };
-    // the positions of a step that a row may see; tiles: which are no holes
-    auto live_of = [&](uint32_t x, uint32_t tiles) -> uint64_t {
-        uint64_t b = 0;
+    uint64_t mine = 0, at = 0;
+    for (uint32_t s0 = 0; s0 < a.n; s0 += T) {
+        uint32_t steps;
+        uint64_t all;
+        mine = count(s0 + threadIdx.x, steps);
+        at = p.total + scan(mine, all);
+        p.total += all;
+        longest = steps > longest ? steps : longest;
+    }
 #pragma unroll
-        for (int t = 0; t < NT; t++) b |= tiles >> t & 1 ? 0xFFFFull << (16 * t) : 0;
-        return b & low_bits((int64_t)h.sq.total - x);
-    };
-    Wave r;
-    uint32_t tiles[RING - 1];  // of the steps under way: which tiles are no holes
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t y = __shfl_xor(longest, d, 64);
+        longest = y > longest ? y : longest;
+    }
+    if (lane == 0) s_long[w] = longest;
+    if (threadIdx.x == 0) s_seq = a.n;
+    __syncthreads();
 #pragma unroll
-    for (int n = 0; n < RING - 1; n++) {
-        tiles[n] = 0;
-        if ((uint32_t)n < steps) {
-            tiles[n] = look(n);
-            issue(n, ring[n]);
+    for (uint32_t k = 0; k < NW; k++) longest = s_long[k] > longest ? s_long[k] : longest;
+    // at most kMaxChunks workgroups share an item
+    const uint64_t even = (p.total + gridDim.x - 1) / gridDim.x;
+    const uint32_t few = (longest + kMaxChunks - 3) / (kMaxChunks - 2);
+    const uint64_t run = even > few ? even : few;
+    p.run = (uint32_t)(run > kLeast ? run : kLeast);
+    const uint64_t start = (uint64_t)wg * p.run;
+    uint64_t sum = 0;
+    for (uint32_t s0 = 0; s0 < a.n; s0 += T) {
+        const uint32_t s = s0 + threadIdx.x;
+        if (a.n > T) {
+            uint32_t steps;
+            uint64_t all;
+            mine = count(s, steps);
+            at = sum + scan(mine, all);
+            sum += all;
+        }
+        if (s < a.n) {
+            if (wg == 0) a.place[1 + s] = at;
+            if (start >= at && start < at + mine) s_seq = s, s_at = start - at;
         }
     }
-    r.init(a, h, rbase);
-    // where the lane reads a stage: K piece 4 ks + j of row c16, V's dims of row 4 j + i; a tile further 16 rows on
-    uint32_t k_at[KS], v_at[4][VW > 4 ? 2 : 1];
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) k_at[ks] = r.c16 * RB + ((4 * ks + r.j) ^ (r.c16 & 7)) * 16;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t row = 4 * r.j + i;
-        if constexpr (VW == 2) v_at[i][0] = HALF + row * RB + ((r.c16 / 2) ^ (row & 7)) * 16 + (r.c16 & 1) * 8;
-        else
-#pragma unroll
-            for (int d = 0; d < VW; d += 4) v_at[i][d / 4] = HALF + row * RB + ((4 * d + r.c16) ^ (row & 7)) * 16;
-    }
-    auto value = [&](const char* stage, int t, int i, uint32_t (&v)[VW]) {
-        if constexpr (VW == 2) {
-            const u2 y = *(const u2*)(stage + v_at[i][0] + t * 16 * RB);
-            v[0] = y[0], v[1] = y[1];
-        } else {
-#pragma unroll
-            for (int d = 0; d < VW; d += 4) {
-                const u4 y = *(const u4*)(stage + v_at[i][d / 4] + t * 16 * RB);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[d + e] = y[e];
-            }
-        }
-    };
-    uint32_t slot = 0;  // n % RING
-    for (uint32_t n = 0; n < steps; n++) {
-        // step n has landed for every wave, and every wave is done with the stage that is filled next
-        if (RING > 2 && n + RING - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * OPS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const uint32_t tl = tiles[0];
-#pragma unroll
-        for (int k = 0; k + 1 < RING - 1; k++) tiles[k] = tiles[k + 1];
-        if (n + RING - 1 < steps) {
-            turn_page(n + RING - 1);
-            tiles[RING - 2] = look(n + RING - 1);
-            issue(n + RING - 1, ring[slot ? slot - 1 : RING - 1]);
-        }
-        const char* stage = ring[slot];
-        slot = slot + 1 < RING ? slot + 1 : 0;
-        if (!busy) continue;
-        const uint32_t x = h.x0 + n * STEP;
-        const bool mk = tl != (1u << NT) - 1 || x + STEP > h.sq.ctx;
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) r.scores(t, ks, *(const u4*)(stage + k_at[ks] + t * 16 * RB));
-        uint64_t lv = 0;
-        if (mk) {
-            lv = live_of(x, tl);
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, lv, rt));
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) r.weigh(rt);
-        uint32_t odd = 0;
-        if constexpr (F32) {
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t v[VW];
-                    value(stage, t, i, v);
-                    if (mk) odd |= r.clean(t, i, lv, v);
-                    r.add32(t, i, v);
-                }
-        } else {
-#pragma unroll
-            for (int g = 0; g < NT / 2; g++) {
-                uint32_t v[2][4][VW];
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) value(stage, 2 * g + t, i, v[t][i]);
-                if (mk) {
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) odd |= r.clean(2 * g + t, i, lv, v[t][i]);
-                }
-                r.add16(g, v[0], v[1]);
-            }
-        }
-        if (mk && __any(odd)) r.poison(a, h, x, lv);
-    }
-    if (!busy) return;  // no barrier follows
-    r.close();
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float y[ND];
-#pragma unroll
-            for (int d = 0; d < ND; d++) y[d] = r.o[rt][d][i];
-            const int from = (int)(4 * r.j + i);  // the lane that holds row 4 j + i's m and sum
-            r.put(a, h, w * 32 + rt * 16 + 4 * r.j + i, __shfl(r.m[rt], from, 64), __shfl(r.l[rt], from, 64), y);
-        }
+    if (wg == 0 && threadIdx.x == 0) a.place[0] = p.run;
+    __syncthreads();
+    seq = s_seq;
+    in_seq = s_at;
+    return p;
 }
 
-// Chunks of a row, joined.  A block takes four rows: a wave weighs a row's chunks (lane = chunk, at most 64),
-// then HD / 4 lanes by SPLIT groups a row add them up, each group every SPLIT-th chunk: two dependent reads of
-// memory in all.  (One thread group walking the chunks of a row: 19.6 us for 33 chunks of 112 rows x 8.)
-template <int HD, bool SPARSE>
+// NW waves side by side in rows, 32 rows each, over steps of NT tiles.  K and V of a step go to LDS, RING - 1 steps
+// ahead; one barrier a step.  A place there holds rows of RB bytes, whose 16-byte pieces lie at their number ^ (row &
+// 7), so that eight lanes that read one piece of eight rows meet eight different bank groups.  Loads write LDS in lane
+// order, so the lane that lands in a place fetches the piece that belongs there.
+#ifndef LK_WIDE_OCC
+#define LK_WIDE_OCC 2
+#endif
+template <int HD, bool F32, int NW>
+struct Wide {
+    static constexpr int NT = F32 || HD == 128 ? 2 : 4, STEP = NT * 16, ROWS = NW * 32;
+};
+template <int HD, bool F32, int NW>
+__global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const LkPagedAttn a) {
+    constexpr int RT = 2, NT = Wide<HD, F32, NW>::NT, STEP = Wide<HD, F32, NW>::STEP, ROWS = Wide<HD, F32, NW>::ROWS;
+    using Wave = Rows<HD, F32, RT, NT, false, !F32>;
+    constexpr int ND = Wave::ND, KS = Wave::KS, VW = Wave::VW, ES = Wave::ES;
+    constexpr int RB = HD * ES, PIECES = RB / 16, PER = 64 / PIECES;  // rows that one load instruction covers
+    constexpr int SIDE = STEP * RB, OPS = SIDE / 1024 / NW;           // a step's K or V; a wave's loads of it
+    constexpr int RING = SIDE * NW <= 8192 * 4 && NW == 4 ? 3 : 2;
+    static_assert(OPS >= 1 && SIDE % (1024 * NW) == 0 && 16 % PER == 0, "whole load instructions, each within a tile");
+    __shared__ __align__(1024) char ring[RING][2 * SIDE];
+    typedef __attribute__((address_space(3))) uint32_t* lptr;
+    typedef __attribute__((address_space(1))) uint32_t* gptr;
+    typedef __attribute__((address_space(3))) s4* sptr;
+    const uint32_t lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // neighbours in the order of work are on one XCD (workgroups go round the 8): row groups of a kv head meet in its L2
+    const uint32_t wg = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    uint32_t seq;
+    uint64_t in_seq;
+    const Plan plan = plan_runs<NW>(a, wg, STEP, ROWS, seq, in_seq);
+    const uint64_t start = (uint64_t)wg * plan.run;
+    if (start >= plan.total) return;  // uniform
+    const uint64_t left64 = plan.total - start;
+    uint32_t left = left64 < plan.run ? (uint32_t)left64 : plan.run;
+
+    while (left) {
+        Share h{};
+        h.s = seq;
+        h.sq = seq_of<false>(a, seq);
+        const uint32_t groups = row_groups(a, h.sq, ROWS), of_item = groups ? item_steps(h.sq, STEP) : 0;
+        if (in_seq >= (uint64_t)groups * a.p.n_kv * of_item) {  // the sequence is done, or has nothing: on to the next
+            seq++;
+            in_seq = 0;
+            continue;
+        }
+        const uint32_t item = (uint32_t)(in_seq / of_item), step0 = (uint32_t)(in_seq - (uint64_t)item * of_item);
+        const uint32_t steps = of_item - step0 < left ? of_item - step0 : left;
+        h.kvh = item / groups;
+        h.row0 = (item - h.kvh * groups) * ROWS;
+        h.R = h.sq.rows * a.G;
+        h.x0 = step0 * STEP;
+        h.x1 = (step0 + steps) * STEP < h.sq.total ? (step0 + steps) * STEP : h.sq.total;
+        h.whole = steps == of_item;
+        // a run has at most one part that began before it and one that goes on behind it
+        h.part = ((size_t)wg * 2 + (step0 == 0)) * ROWS;
+        left -= steps;
+        in_seq += steps;
+        const uint32_t rbase = h.row0 + w * 32;
+        const bool busy = rbase < h.R;  // wave-uniform; an idle wave loads with the others
+
+        // Where the part's tiles lie, 64 at a time, one a lane (byte of the first row), and which are no holes; `ahead`:
+        // page ids of the next 64.
+        auto ids_of = [&](uint32_t block) LK_INLINE -> uint32_t {
+            uint32_t pos;
+            const uint64_t y = (uint64_t)h.x0 + ((uint64_t)block * 64 + lane) * 16;
+            return y < h.x1 ? tile_page<false>(a, h, (uint32_t)y, pos) : LK_NO_PAGE;
+        };
+        uint32_t at_lo, at_hi, block = 0;
+        uint64_t there;
+        auto place = [&](uint32_t id) LK_INLINE {
+            const uint64_t at = tile_base(a, h, id, h.x0 + (block * 64 + lane) * 16, HD) * ES;
+            at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
+            there = __ballot(id < a.p.n_pages);
+        };
+        place(ids_of(0));
+        uint32_t ahead = ids_of(1);
+        // this lane's piece of an instruction's rows: the instruction's first row is a multiple of PER
+        const uint32_t in_op = lane / PIECES, my_piece = lane % PIECES;
+        auto issue = [&](uint32_t n, char* to) LK_INLINE {
+#pragma unroll
+            for (int k = 0; k < 2 * OPS; k++) {
+                const uint32_t q = w * OPS + k % OPS, row0 = q * PER, tile = (n * NT + row0 / 16) & 63;
+                const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, tile) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, tile);
+                const uint32_t mine = ((row0 & 15) + in_op) * RB + ((my_piece ^ ((row0 + in_op) & 7)) * 16);
+                const char* from = (const char*)(k < OPS ? a.p.k : a.p.v) + at;
+                __builtin_amdgcn_global_load_lds((gptr)(from + mine), (lptr)(to + (k < OPS ? 0 : SIDE) + q * 1024), 16, 0, 0);
+            }
+        };
+        // before a step's issue: the next 64 tiles begin every 64 / NT steps
+        auto turn_page = [&](uint32_t n) LK_INLINE {
+            if (n * NT / 64 != block) {
+                block++;
+                place(ahead);
+                ahead = ids_of(block + 1);
+            }
+        };
+        auto look = [&](uint32_t n) LK_INLINE -> uint32_t { return (uint32_t)(there >> (n * NT & 63)) & ((1u << NT) - 1); };
+        // the positions of a step that a row may see; tiles: which are no holes
+        auto live_of = [&](uint32_t x, uint32_t tiles) LK_INLINE -> uint64_t {
+            uint64_t b = 0;
+#pragma unroll
+            for (int t = 0; t < NT; t++) b |= tiles >> t & 1 ? 0xFFFFull << (16 * t) : 0;
+            return b & low_bits((int64_t)h.sq.total - x);
+        };
+        asm volatile("s_barrier" ::: "memory");  // the last part's stages are read
+        uint32_t tiles[RING - 1];  // of the steps under way: which tiles are no holes
+#pragma unroll
+        for (int n = 0; n < RING - 1; n++) {
+            tiles[n] = 0;
+            if ((uint32_t)n < steps) {
+                tiles[n] = look(n);
+                issue(n, ring[n]);
+            }
+        }
+        Wave r;
+        const bool scaled = r.init(a, h, rbase);
+        // Where the lane reads a stage: K piece 4 ks + j of row c16; V f32: its dims of row 4 j + i, V f16: the part of
+        // column tile d that it hands the transposing read (of 16 lanes, four hold a row's 16 dims, and each gets one
+        // dim of the four rows).  A tile further is 16 rows on.
+        uint32_t k_at[KS], v_at[F32 ? 4 : ND][VW > 4 ? 2 : 1];
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) k_at[ks] = r.c16 * RB + ((4 * ks + r.j) ^ (r.c16 & 7)) * 16;
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t row = 4 * r.j + i;
+#pragma unroll
+                for (int d = 0; d < VW; d += 4) v_at[i][d / 4] = SIDE + row * RB + ((4 * d + r.c16) ^ (row & 7)) * 16;
+            }
+        } else {
+            const uint32_t row = 4 * r.j + r.c16 / 4;
+#pragma unroll
+            for (int d = 0; d < ND; d++) v_at[d][0] = SIDE + row * RB + ((2 * d + r.c16 % 4 / 2) ^ (row & 7)) * 16 + (r.c16 & 1) * 8;
+        }
+        uint32_t slot = 0;  // n % RING
+        for (uint32_t n = 0; n < steps; n++) {
+            // step n has landed for every wave, and every wave is done with the stage that is filled next
+            if (RING > 2 && n + RING - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * 2 * OPS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            const uint32_t tl = tiles[0];
+#pragma unroll
+            for (int k = 0; k + 1 < RING - 1; k++) tiles[k] = tiles[k + 1];
+            if (n + RING - 1 < steps) {
+                turn_page(n + RING - 1);
+                tiles[RING - 2] = look(n + RING - 1);
+                issue(n + RING - 1, ring[slot ? slot - 1 : RING - 1]);
+            }
+            char* stage = ring[slot];
+            slot = slot + 1 < RING ? slot + 1 : 0;
+            const uint32_t x = h.x0 + n * STEP;
+            const bool masked = tl != (1u << NT) - 1 || x + STEP > h.sq.ctx;  // uniform: something to hide
+            uint64_t live = 0;
+            bool odd = false;
+            if (masked) {
+                // V of positions that no row sees becomes zero, and what is not finite too
+                live = live_of(x, tl);
+                uint32_t any = 0;
+                for (uint32_t p = threadIdx.x; p < SIDE / 16; p += NW * 64) {
+                    u4* at = (u4*)(stage + SIDE + p * 16);
+                    u4 y = *at;
+                    const bool see = live >> (p / PIECES) & 1;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] = Wave::clean_word(see ? y[e] : 0, any);
+                    *at = y;
+                }
+                odd = __syncthreads_or(any != 0);
+            }
+            if (!busy) continue;
+            f4 sc[RT][NT];
+            {
+                u4 kr[NT][KS];
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++) kr[t][ks] = *(const u4*)(stage + k_at[ks] + t * 16 * RB);
+                r.scores(kr, sc);
+            }
+            if (masked) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt), sc);
+                if (odd) r.poison(a, h, x, live);
+            }
+            r.move(sc, scaled);
+            if constexpr (F32) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t y[VW];
+#pragma unroll
+                        for (int d = 0; d < VW; d += 4) {
+                            const u4 z = *(const u4*)(stage + v_at[i][d / 4] + t * 16 * RB);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) y[d + e] = z[e];
+                        }
+                        r.add32(sc, t, i, y);
+                    }
+            } else {
+#pragma unroll
+                for (int g = 0; g < NT / 2; g++) {
+                    h8 vb[ND];
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        u2 y[2];
+#pragma unroll
+                        for (int t = 0; t < 2; t++)
+                            y[t] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((sptr)(stage + v_at[d][0] + (2 * g + t) * 16 * RB)));
+                        vb[d] = __builtin_bit_cast(h8, u4{y[0][0], y[0][1], y[1][0], y[1][1]});
+                    }
+                    r.add16(sc, g, vb);
+                }
+            }
+        }
+        if (!busy) continue;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float y[ND];
+#pragma unroll
+                for (int d = 0; d < ND; d++) y[d] = r.o[rt][d][i];
+                const float top = r.max_of(rt, i), sum = r.sum_of(rt, i);
+                r.put(a, h, w * 32 + rt * 16 + 4 * r.j + i, top, sum, y);
+            }
+    }
+}
+
+// Parts of a row, joined.  A block takes four rows: a wave weighs a row's parts (lane = part, at most 64), then HD / 4
+// lanes by SPLIT groups a row add them up, each group every SPLIT-th part: two dependent reads of memory in all.  (One
+// thread group walking the parts of a row: 19.6 us for 33 parts of 112 rows x 8.)  ROWS: of a workgroup of the wide
+// kernel; 0: parts are the narrow kernel's chunks.
+template <int HD, bool SPARSE, int ROWS, int STEP>
 __global__ __launch_bounds__(256) void paged_fold_kernel(const LkPagedAttn a) {
     constexpr uint32_t L = HD / 4, SPLIT = 64 / L;
     __shared__ float s_f[4][kMaxChunks];
     __shared__ __align__(16) f4 s_y[4][SPLIT][L];
     const uint32_t pair = blockIdx.x, kvh = pair % a.p.n_kv, s = pair / a.p.n_kv;
     const Seq sq = seq_of<SPARSE>(a, s);
-    const uint32_t nch = chunks_of(sq.total, a.chunk), R = sq.rows * a.G;
-    if (!sq.live || nch == 1 || blockIdx.y * 4 >= R) return;  // uniform
-    const uint32_t w = threadIdx.x >> 6, lane = threadIdx.x & 63, row = blockIdx.y * 4 + w;
-    const size_t base = (size_t)pair * a.n_chunks * a.rows_pad + row;
+    const uint32_t R = sq.rows * a.G, w = threadIdx.x >> 6, lane = threadIdx.x & 63, row = blockIdx.y * 4 + w;
+    if (!sq.live || blockIdx.y * 4 >= R) return;  // uniform
+    uint32_t parts;
+    size_t base, stride;  // of the row's parts, but for the wide kernel's first
+    if constexpr (ROWS) {
+        const uint32_t groups = row_groups(a, sq, ROWS), of_item = item_steps(sq, STEP), run = (uint32_t)a.place[0];
+        const uint64_t at = a.place[1 + s] + (uint64_t)(kvh * groups + blockIdx.y * 4 / ROWS) * of_item;
+        const uint64_t wg = at / run;
+        parts = (uint32_t)((at + of_item - 1) / run - wg) + 1;
+        base = wg * 2 * ROWS + row % ROWS;
+        stride = 2 * ROWS;
+    } else {
+        parts = chunks_of(sq.total, a.chunk);
+        base = (size_t)pair * a.n_chunks * a.rows_pad + row;
+        stride = a.rows_pad;
+    }
+    if (parts == 1) return;  // uniform: written as it is
+    auto at = [&](uint32_t k) LK_INLINE { return base + k * stride + (ROWS && k == 0 ? ROWS : 0); };
     if (row < R) {  // wave-uniform
         float2 ml{-INFINITY, 0.f};
-        if (lane < nch) ml = *(const float2*)(a.part_ml + 2 * (base + (size_t)lane * a.rows_pad));
+        if (lane < parts) ml = *(const float2*)(a.part_ml + 2 * at(lane));
         const float top = lk_wave_max(ml.x), f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
         const float sum = lk_wave_sum(ml.y * f);
         s_f[w][lane] = f * (sum == 0.f ? 0.f : 1.f / sum);
@@ -761,19 +998,22 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const LkPagedAttn a) {
     f4 y = f4{0.f, 0.f, 0.f, 0.f};
     if (row < R) {
 #pragma unroll 4
-        for (uint32_t k = sp; k < nch; k += SPLIT)
-            y += *(const f4*)(a.part_o + (base + (size_t)k * a.rows_pad) * HD + 4 * c) * s_f[w][k];
+        for (uint32_t k = sp; k < parts; k += SPLIT) y += *(const f4*)(a.part_o + at(k) * HD + 4 * c) * s_f[w][k];
     }
     s_y[w][sp][c] = y;
     __syncthreads();
     if (row >= R || sp) return;
 #pragma unroll
     for (uint32_t k = 1; k < SPLIT; k++) y += s_y[w][k][c];
-    *(f4*)(a.out + (((size_t)s * a.tokens + row / a.G) * a.n_heads + kvh * a.G + row % a.G) * HD + 4 * c) = y;
+    const uint32_t t = row / a.G;
+    *(f4*)(a.out + (((size_t)s * a.tokens + t) * a.n_heads + kvh * a.G + row - t * a.G) * HD + 4 * c) = y;
 }
 
 }  // namespace
 
+// Narrow: enough chunks of the table's capacity to fill the card.  Wide: as many workgroups as it holds, each with two
+// places for parts.
+constexpr uint32_t kCus = 256;
 LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32_t n_kv, uint32_t rows,
                           uint64_t positions) {
     LkPagedPlan p{};
@@ -784,46 +1024,59 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
     p.n_rg = (rows + per - 1) / per;
     p.rows_pad = p.n_rg * per;
     const uint64_t base = (uint64_t)n * n_kv * p.n_rg;
-    const uint32_t step = p.narrow ? (f32 || hd == 128 ? 32 : 64) * 4 : 64;  // narrow: every wave has a step
-    const uint64_t steps = (positions + step - 1) / step;
-    const uint64_t aim = p.narrow ? 1024 : LK_WIDE_AIM, few = LK_WIDE_FEW, least = LK_WIDE_LEAST;
-    uint64_t c = (aim + base - 1) / base;
-    if (!p.narrow && c > 1) {  // long chunks, unless there are few
-        const uint64_t by_len = (positions + least - 1) / least, by_fill = (few + base - 1) / base;
-        const uint64_t most = by_len > by_fill ? by_len : by_fill;
-        c = c < most ? c : most;
+    const uint32_t step = f32 || hd == 128 ? 32 : 64;
+    if (p.narrow) {
+        const uint32_t all = step * 4;  // every wave has a step
+        const uint64_t steps = (positions + all - 1) / all;
+        uint64_t c = (1024 + base - 1) / base;
+        c = c > kMaxChunks ? kMaxChunks : c;
+        c = c > steps ? steps : c;
+        if (c < 1) c = 1;
+        p.chunk = (uint32_t)((steps + c - 1) / c * all);
+        if (!p.chunk) p.chunk = all;
+        p.n_chunks = (uint32_t)((positions + p.chunk - 1) / p.chunk);
+        if (!p.n_chunks) p.n_chunks = 1;
+        const uint64_t items = (uint64_t)n * n_kv * p.n_chunks;
+        p.blocks = (items + 7) / 8 * 8 * p.n_rg;
+        p.part_rows = p.n_chunks > 1 ? items * p.rows_pad : 0;
+    } else {
+        const uint64_t steps = base * ((positions + step - 1) / step), most = (steps + kLeast - 1) / kLeast;
+        const uint64_t fill = (uint64_t)kCus * LK_WIDE_OCC * 4 / p.waves;
+        p.blocks = ((fill < most ? fill : most) + 7) / 8 * 8;
+        p.part_rows = p.blocks * 2 * per;
+        p.place_bytes = ((uint64_t)n + 1) * 8;
+        p.place_bytes = (p.place_bytes + 255) / 256 * 256;
     }
-    c = c > kMaxChunks ? kMaxChunks : c;
-    c = c > steps ? steps : c;
-    if (c < 1) c = 1;
-    p.chunk = (uint32_t)((steps + c - 1) / c * step);
-    if (!p.chunk) p.chunk = step;
-    p.n_chunks = (uint32_t)((positions + p.chunk - 1) / p.chunk);
-    if (!p.n_chunks) p.n_chunks = 1;
-    const uint64_t items = (uint64_t)n * n_kv * p.n_chunks;
-    p.blocks = (items + 7) / 8 * 8 * p.n_rg;
-    p.part_bytes = p.n_chunks > 1 ? items * p.rows_pad * (hd + 2) * 4 : 0;
+    p.part_bytes = p.place_bytes + p.part_rows * (hd + 2) * 4;
     return p;
 }
 
 template <int HD, bool F32, bool SPARSE>
 static hipError_t launch(const LkPagedAttn& a, const LkPagedPlan& p, hipStream_t st) {
-    const dim3 grid((uint32_t)p.blocks);
+    const dim3 grid((uint32_t)p.blocks), fold(a.n * a.p.n_kv, (a.tokens * a.G + 3) / 4);
     if (p.narrow) {
         if (p.tiles == 1) hipLaunchKernelGGL((paged_narrow_kernel<HD, F32, 1, SPARSE>), grid, dim3(256), 0, st, a);
         else if (!SPARSE) hipLaunchKernelGGL((paged_narrow_kernel<HD, F32, 2, false>), grid, dim3(256), 0, st, a);
         else return hipErrorInvalidValue;
-    } else if (SPARSE) {
-        return hipErrorInvalidValue;
-    } else if (p.waves == 2) {
-        hipLaunchKernelGGL((paged_wide_kernel<HD, F32, 2>), grid, dim3(128), 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || p.n_chunks == 1) return e;
+        hipLaunchKernelGGL((paged_fold_kernel<HD, SPARSE, 0, 0>), fold, dim3(256), 0, st, a);
+    } else if constexpr (!SPARSE) {
+#define LK_WIDE(NW)                                                                                                   \
+    hipLaunchKernelGGL((paged_wide_kernel<HD, F32, NW>), grid, dim3(NW * 64), 0, st, a);                              \
+    const hipError_t e = hipGetLastError();                                                                           \
+    if (e != hipSuccess) return e;                                                                                    \
+    hipLaunchKernelGGL((paged_fold_kernel<HD, false, Wide<HD, F32, NW>::ROWS, Wide<HD, F32, NW>::STEP>), fold,        \
+                       dim3(256), 0, st, a)
+        if (p.waves == 2) {
+            LK_WIDE(2);
+        } else {
+            LK_WIDE(4);
+        }
+#undef LK_WIDE
     } else {
-        hipLaunchKernelGGL((paged_wide_kernel<HD, F32, 4>), grid, dim3(256), 0, st, a);
+        return hipErrorInvalidValue;
     }
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.n_chunks == 1) return e;
-    hipLaunchKernelGGL((paged_fold_kernel<HD, SPARSE>), dim3(a.n * a.p.n_kv, (a.tokens * a.G + 3) / 4), dim3(256), 0, st,
-                       a);
     return hipGetLastError();
 }
 
@@ -833,10 +1086,9 @@ hipError_t lk_paged_attn_launch(LkPagedAttn a, const LkPagedPlan& p, void* ws, h
     a.n_rg = p.n_rg;
     a.rows_pad = p.rows_pad;
     a.scale = 1.44269504088896340736f * (a.p.hd == 64 ? 0.125f : 0.08838834764831845f);
-    if (p.n_chunks > 1) {
-        a.part_o = (float*)ws;
-        a.part_ml = a.part_o + (size_t)a.n * a.p.n_kv * p.n_chunks * p.rows_pad * a.p.hd;
-    }
+    a.place = (uint64_t*)ws;
+    a.part_o = (float*)((char*)ws + p.place_bytes);
+    a.part_ml = a.part_o + p.part_rows * a.p.hd;
 #define LK_PAGED(HD, F32) (a.sel ? launch<HD, F32, true>(a, p, st) : launch<HD, F32, false>(a, p, st))
     if (a.p.hd == 64) return a.p.f32 ? LK_PAGED(64, true) : LK_PAGED(64, false);
     return a.p.f32 ? LK_PAGED(128, true) : LK_PAGED(128, false);

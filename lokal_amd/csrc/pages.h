@@ -61,6 +61,7 @@ struct LkPagedAttn {
     uint32_t take;
     // set by the launch
     float *part_ml, *part_o;
+    uint64_t* place;       // wide: steps of a run, then where each sequence's steps begin
     uint32_t chunk;        // positions of a chunk
     uint32_t n_chunks, n_rg, rows_pad;
     float scale;           // log2(e) / sqrt(hd)
@@ -70,7 +71,7 @@ struct LkPagedPlan {
     uint32_t tiles, waves; // 16-row tiles of a wave, waves of a workgroup
     uint32_t chunk, n_chunks, n_rg, rows_pad;
     uint64_t blocks;
-    uint64_t part_bytes;
+    uint64_t place_bytes, part_rows, part_bytes;
 };
 // positions: the most that a sequence can show (its table's capacity; sparse: take pages)
 LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32_t n_kv, uint32_t rows, uint64_t positions);
