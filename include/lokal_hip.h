@@ -448,7 +448,8 @@ int lkhip_page_bounds(const lkhip_kv_pages* pages, const lkhip_page_table* table
  * head: the first n_first, the last n_last, and of the others those whose
  * bounds (lkhip_page_bounds) let a q.k be largest, i.e. by
  * max over the kv head's query heads of sum_d max(q_d * min_d, q_d * max_d),
- * taken in f64; a NaN counts as largest, equal ones go to the lowest page.
+ * taken in f64; a page with a bound that is not finite counts as largest, equal
+ * ones go to the lowest page.
  * n_first + n_last <= n_take.  taken: [n][n_kv_heads][n_take] page numbers
  * within the sequence (not ids), ascending, LKHIP_NO_PAGE behind the last; a
  * sequence of at most n_take pages is read whole.  q, out: [n][n_heads *

@@ -7,9 +7,9 @@ namespace {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// A number as an unsigned key of the same order, NaN above all.
+// A number as an unsigned key of the same order, above all where it is not finite.
 __device__ __forceinline__ uint64_t order_key(double x) {
-    if (x != x) return ~0ull;
+    if (!(fabs(x) < (double)INFINITY)) return ~0ull;
     const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);  // -0 as 0
     return b >> 63 ? ~b : b | 1ull << 63;
 }
@@ -18,7 +18,8 @@ __device__ __forceinline__ uint64_t order_key(double x) {
 // which no q.k of the page exceeds; products of f32 and f16 are exact in 64 bits and
 // their sums wrong by 2^-52, so that which page is taken does not hang on the order of
 // a sum (f64 products run at the f32 rate here).  Eight lanes take a page, E = HD / 8
-// dims each; which bound a dim needs hangs on its q alone.
+// dims each, as max(q, 0) hi + min(q, 0) lo: two products a dim and head, the bounds
+// widened once for all heads.  A bound that is not finite makes the sum so too.
 template <int N>
 __device__ __forceinline__ double dpp_add(double x) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
@@ -43,19 +44,14 @@ struct PageBounds {
             for (int e = 0; e < 4; e++) lo[4 * w + e] = x[e], hi[4 * w + e] = y[e];
         }
     }
-    // q: the lane's E dims
-    __device__ __forceinline__ double score(const double* q) const {
-        double sum = 0;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const double y = q[e];
-            const bool up = y > 0;
-            float f;
-            if constexpr (sizeof(KV) == 4) f = __uint_as_float(up ? hi[e] : lo[e]);
-            else f = lk_h2f((uint16_t)((up ? hi[e / 2] : lo[e / 2]) >> (16 * (e & 1))));
-            sum = fma(y, (double)f, sum);
-        }
-        return sum8(sum);
+    // The bounds of dim e of the lane.
+    __device__ __forceinline__ double low(int e) const {
+        if constexpr (sizeof(KV) == 4) return (double)__uint_as_float(lo[e]);
+        else return (double)lk_h2f((uint16_t)(lo[e / 2] >> (16 * (e & 1))));
+    }
+    __device__ __forceinline__ double high(int e) const {
+        if constexpr (sizeof(KV) == 4) return (double)__uint_as_float(hi[e]);
+        else return (double)lk_h2f((uint16_t)(hi[e / 2] >> (16 * (e & 1))));
     }
 };
 
@@ -91,11 +87,17 @@ __device__ __forceinline__ void score_pages(const LkSparse& a, uint32_t s, uint3
             if (id < a.p.n_pages) {
                 PageBounds<KV, HD> b;
                 b.load(a.bounds, a.p, id, kvh, c);
-                for (uint32_t g = 0; g < gn; g++) {
-                    double y[E];
+                double bl[E], bh[E];
 #pragma unroll
-                    for (int e = 0; e < E; e++) y[e] = s_q[g * HD + c * E + e];
-                    const uint64_t k = order_key(b.score(y));
+                for (int e = 0; e < E; e++) bl[e] = b.low(e), bh[e] = b.high(e);
+                for (uint32_t g = 0; g < gn; g++) {
+                    double sum = 0;
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const double y = s_q[g * HD + c * E + e];
+                        sum = fma(fmax(y, 0.0), bh[e], fma(fmin(y, 0.0), bl[e], sum));
+                    }
+                    const uint64_t k = order_key(sum8(sum));
                     key = k > key ? k : key;
                 }
             }
@@ -121,8 +123,11 @@ __global__ __launch_bounds__(256) void sparse_score_kernel(const LkSparse a) {
 // pages above it and the first of those at it, in order: equal keys go to the lowest
 // page.  One workgroup a (sequence, kv head); FUSED: it takes the scores itself and
 // keeps the keys in LDS.  (A thread that walks 256 bins eight times: 62-78 us.)
-constexpr uint32_t kChoose = 1024, kBins = 2048, kFusedPages = 4096;
-template <typename KV, int HD, bool FUSED>
+#ifndef LK_FUSED_PAGES
+#define LK_FUSED_PAGES 256
+#endif
+constexpr uint32_t kBins = 2048, kFusedPages = LK_FUSED_PAGES;
+template <typename KV, int HD, bool FUSED, uint32_t kChoose>
 __global__ __launch_bounds__(kChoose) void sparse_choose_kernel(const LkSparse a) {
     __shared__ uint32_t s_bin[kBins], s_part[kChoose / 64], s_find[3];
     __shared__ uint64_t s_and[kChoose / 64], s_or[kChoose / 64];
@@ -197,15 +202,22 @@ __global__ __launch_bounds__(kChoose) void sparse_choose_kernel(const LkSparse a
             if (asked(x, k)) atomicAdd(&s_bin[(uint32_t)(k >> sh) & (kBins - 1)], 1u);
         }
         __syncthreads();
-        // thread t holds the bins 2 t' and 2 t' + 1 counted from the top
-        const uint32_t b1 = kBins - 1 - 2 * tid, c1 = s_bin[b1], c0 = s_bin[b1 - 1];
-        uint32_t total;
-        const uint32_t above = scan(c1 + c0, total);
-        if (above < want && above + c1 + c0 >= want) {  // one thread
-            const bool lower = above + c1 < want;
-            s_find[0] = lower ? b1 - 1 : b1;
-            s_find[1] = lower ? above + c1 : above;
-            s_find[2] = lower ? c0 : c1;
+        // thread t holds OF neighbouring bins, counted from the top
+        constexpr uint32_t OF = kBins / kChoose;
+        uint32_t c[OF], sum = 0, total;
+#pragma unroll
+        for (uint32_t k = 0; k < OF; k++) c[k] = s_bin[kBins - 1 - OF * tid - k], sum += c[k];
+        uint32_t above = scan(sum, total);
+        if (above < want && above + sum >= want) {  // one thread
+#pragma unroll
+            for (uint32_t k = 0; k < OF; k++) {
+                if (above < want && above + c[k] >= want) {
+                    s_find[0] = kBins - 1 - OF * tid - k;
+                    s_find[1] = above;
+                    s_find[2] = c[k];
+                }
+                above += c[k];
+            }
         }
         __syncthreads();
         const uint32_t bin = s_find[0], count = s_find[2];
@@ -243,14 +255,15 @@ template <typename KV, int HD>
 static void select_launch(const LkSparse& a, hipStream_t st) {
     const dim3 pairs(a.p.n_kv, a.n);
     if (a.t.max_pages <= kFusedPages) {
-        hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, true>), pairs, dim3(kChoose), 0, st, a);
+        hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, true, 256>), pairs, dim3(256), 0, st, a);
         return;
     }
     uint32_t blocks = 2048 / (a.n * a.p.n_kv) + 1;
     const uint32_t most = (a.t.max_pages + 31) / 32;
     if (blocks > most) blocks = most;
     hipLaunchKernelGGL((sparse_score_kernel<KV, HD>), dim3(blocks, a.p.n_kv, a.n), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, false>), pairs, dim3(kChoose), 0, st, a);
+    if (a.t.max_pages <= 2048) hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, false, 256>), pairs, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, false, 1024>), pairs, dim3(1024), 0, st, a);
 }
 hipError_t lk_sparse_select_launch(const LkSparse& a, hipStream_t st) {
     if (a.p.f32) a.p.hd == 64 ? select_launch<float, 64>(a, st) : select_launch<float, 128>(a, st);

@@ -199,9 +199,9 @@ static int plan_of(const LkPages& p, const LkTable& t, size_t n, size_t tokens, 
     keys = take ? (size_t)n * p.n_kv * t.max_pages * 8 : 0;
     keys = (keys + 255) / 256 * 256;
     bytes = keys + plan.part_bytes;
-    if (plan.blocks > 0x7FFFFFFF || (uint64_t)n * p.n_kv * plan.n_chunks > 0x7FFFFFFF)
-        return fail(LKHIP_E_INVALID, "%s: %zu sequences x %zu tokens x %zu heads are too many for one call", who, n,
-                    tokens, n_heads);
+    if (plan.blocks > 0x7FFFFFFF || (uint64_t)n * p.n_kv * (plan.n_chunks + 1) > 0x7FFFFFFF || plan.steps > 0xFFFFFFFF)
+        return fail(LKHIP_E_INVALID, "%s: %zu sequences x %zu tokens x %zu heads over %llu positions are too many for one call",
+                    who, n, tokens, n_heads, (unsigned long long)cap);
     return LKHIP_OK;
 }
 static int ws_check(const void* ws, size_t have, size_t need, const char* who) {

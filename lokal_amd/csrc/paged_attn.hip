@@ -223,40 +223,36 @@ struct Rows {
         return scaled;
     }
 
-    // Scores relative to m: the products start at -m.  k: f16 the lane's 8 dims 32 ks + 8 j of position c16, f32 its 4
-    // dims 16 ks + 4 j.  Products that follow each other belong to different sums.
-    __device__ __forceinline__ void scores(const u4 (&k)[NT][KS], Scores& sc) const {
-        f4 c[RT];
+    // Scores relative to m: the products start at -m.
+    __device__ __forceinline__ void start(Scores& sc) const {
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             float z = m[rt] == -INFINITY ? 0.f : -m[rt];
             if constexpr (!F32) z = ldexpf(z, up[rt]);
-            c[rt] = f4{z, z, z, z};
+#pragma unroll
+            for (int t = 0; t < NT; t++) sc[rt][t] = f4{z, z, z, z};
         }
+    }
+    // k: f16 the lane's 8 dims 32 ks + 8 j of position c16, f32 its 4 dims 16 ks + 4 j.  Products that follow each other
+    // belong to different sums.
+    __device__ __forceinline__ void scores(const u4 (&k)[NT], int ks, Scores& sc) const {
+        if constexpr (F32) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            if constexpr (F32) {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++)
-                            sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, k[t][ks])[e], qf[rt][ks][e],
-                                                                             ks == 0 && e == 0 ? c[rt] : sc[rt][t], 0, 0, 0);
-            } else {
+            for (int e = 0; e < 4; e++)
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++)
-                        sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, k[t][ks]), qh[rt][ks],
-                                                                           ks == 0 ? c[rt] : sc[rt][t], 0, 0, 0);
+                        sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, k[t])[e], qf[rt][ks][e], sc[rt][t], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int part = 0; part < 2; part++)
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++)
-                        sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, k[t][ks]), ql[rt][ks], sc[rt][t], 0, 0, 0);
-            }
+                        sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, k[t]), part ? ql[rt][ks] : qh[rt][ks],
+                                                                           sc[rt][t], 0, 0, 0);
         }
     }
 
@@ -332,9 +328,9 @@ struct Rows {
         }
     }
 
-    // f16: tiles 2 g and 2 g + 1.  vb[d]: column tile d of their V, positions 4 j + i of the one, then of the other
-    __device__ __forceinline__ void add16(const Scores& sc, int g, const h8 (&vb)[ND]) {
-        h8 ph[RT], pl[RT], ones;
+    // f16: the weights of tiles 2 g and 2 g + 1 in two parts, and their sums.
+    __device__ __forceinline__ void weights(const Scores& sc, int g, h8 (&ph)[RT], h8 (&pl)[RT]) {
+        h8 ones;
 #pragma unroll
         for (int e = 0; e < 8; e++) ones[e] = (_Float16)1.f;
         float minus = -1.f;  // a register: p - hi is then one mixed product, hi not widened first
@@ -355,15 +351,20 @@ struct Rows {
             pl[rt] = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
         }
 #pragma unroll
-        for (int part = 0; part < 2; part++) {
+        for (int rt = 0; rt < RT; rt++) lr[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[rt], ones, lr[rt], 0, 0, 0);
 #pragma unroll
-            for (int d = 0; d < ND; d++)
+        for (int rt = 0; rt < RT; rt++) lr[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[rt], ones, lr[rt], 0, 0, 0);
+    }
+    // vb: column tiles d0.. of their V, positions 4 j + i of the one tile, then of the other
+    template <int N>
+    __device__ __forceinline__ void add16(const h8 (&ph)[RT], const h8 (&pl)[RT], const h8 (&vb)[N], int d0) {
+#pragma unroll
+        for (int part = 0; part < 2; part++)
+#pragma unroll
+            for (int d = 0; d < N; d++)
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++)
-                    o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part ? pl[rt] : ph[rt], vb[d], o[rt][d], 0, 0, 0);
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) lr[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part ? pl[rt] : ph[rt], ones, lr[rt], 0, 0, 0);
-        }
+                    o[rt][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part ? pl[rt] : ph[rt], vb[d], o[rt][d0 + d], 0, 0, 0);
     }
     __device__ __forceinline__ void add32(const Scores& sc, int t, int i, const uint32_t (&v)[VW]) {
         float p[RT];
@@ -402,8 +403,19 @@ struct Rows {
         }
         return odd;
     }
-    // Rows that see a value that is not finite: NaN in its dim.  Rare, so short: a position at a time.
-    __device__ __forceinline__ void poison(const LkPagedAttn& a, const Share& h, uint32_t x, uint64_t live) {
+    // Rows that see a value that is not finite, in a step that had something to hide: NaN in its dim.  Rare, so short: a
+    // position at a time, after all steps.
+    __device__ __forceinline__ void poison(const LkPagedAttn& a, const Share& h, uint32_t x) {
+        uint64_t live = 0;
+        bool masked = false;
+        for (uint32_t t = 0; t < NT; t++) {
+            uint32_t pos;
+            const uint32_t id = tile_page<SPARSE>(a, h, x + 16 * t, pos);
+            const uint32_t end = SPARSE ? h.sq.ctx : h.sq.total;
+            if (id < a.p.n_pages) live |= (low_bits((int64_t)end - pos) & 0xFFFF) << (16 * t);
+            masked |= id >= a.p.n_pages || pos + 16 > h.sq.ctx;
+        }
+        if (!masked) return;
         for (uint32_t p = 0; p < NT * 16; p++) {
             if (!(live >> p & 1)) continue;  // uniform
             uint32_t pos;
@@ -527,18 +539,24 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
                 }
             }
     };
+    uint32_t odd = 0;
     auto use = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t live, bool masked) LK_INLINE {
         f4 sc[RT][NT];
-        r.scores(k, sc);
+        r.start(sc);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            u4 kk[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) kk[t] = k[t][ks];
+            r.scores(kk, ks, sc);
+        }
         if (__builtin_amdgcn_readfirstlane(masked)) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt), sc);
-            uint32_t odd = 0;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) odd |= r.clean(t, i, live, v[t][i]);
-            if (__any(odd)) r.poison(a, h, x, live);
         }
         r.move(sc, scaled);
         if constexpr (F32) {
@@ -559,7 +577,9 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
                         y[e] = __builtin_amdgcn_perm(v[2 * g + e / 2][2 * (e & 1) + 1][d / 2], v[2 * g + e / 2][2 * (e & 1)][d / 2], pick);
                     vb[d] = __builtin_bit_cast(h8, y);
                 }
-                r.add16(sc, g, vb);
+                h8 ph[RT], pl[RT];
+                r.weights(sc, g, ph, pl);
+                r.add16(ph, pl, vb, 0);
             }
         }
     };
@@ -579,6 +599,8 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
         use(x, kr[1], vr[1], live[1], masked[1]);
         x = nx;
     }
+    if (!SPARSE && __any(odd))
+        for (x = h.x0 + w * STEP; x < h.x1; x += W * STEP) r.poison(a, h, x);
     // ---- the waves join: m and sum per row, then O one wave after the other
 #pragma unroll
     for (int rt = 0; rt < RT; rt++)
@@ -629,8 +651,7 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
 // may end one item and begin others.  Fixed chunks of the table's capacity left half the card idle behind the last
 // of 565 live workgroups on 512 places (8 x 64 tokens over up to 32768 positions: 214 us).
 struct Plan {
-    uint64_t total;
-    uint32_t run;  // steps of a workgroup
+    uint32_t total, run;  // steps in all (the host keeps them below 2^32) and of a workgroup
 };
 // Steps of one item of a sequence, and its items.
 __device__ __forceinline__ uint32_t item_steps(const Seq& q, uint32_t step) { return (q.total + step - 1) / step; }
@@ -646,35 +667,32 @@ constexpr uint32_t kLeast = LK_LEAST;  // steps of a run at least
 // the place) unless one round of the threads holds them.  Workgroup 0 leaves the sequences' places for the fold.
 template <int NW>
 __device__ __forceinline__ Plan plan_runs(const LkPagedAttn& a, uint32_t wg, uint32_t step, uint32_t rows, uint32_t& seq,
-                                          uint64_t& in_seq) {
+                                          uint32_t& in_seq) {
     constexpr uint32_t T = NW * 64;
-    __shared__ uint64_t s_sum[NW];
-    __shared__ uint32_t s_long[NW];
-    __shared__ uint64_t s_at;
-    __shared__ uint32_t s_seq;
+    __shared__ uint32_t s_sum[NW], s_long[NW], s_at, s_seq;
     const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     Plan p{};
     uint32_t longest = 0;
-    auto count = [&](uint32_t s, uint32_t& steps) LK_INLINE -> uint64_t {
+    auto count = [&](uint32_t s, uint32_t& steps) LK_INLINE -> uint32_t {
         steps = 0;
         if (s >= a.n) return 0;
         const Seq q = seq_of<false>(a, s);
         const uint32_t g = row_groups(a, q, rows);
         steps = g ? item_steps(q, step) : 0;
-        return (uint64_t)g * a.p.n_kv * steps;
+        return g * a.p.n_kv * steps;
     };
     // exclusive sum over the block, and the sum
-    auto scan = [&](uint64_t v, uint64_t& all) LK_INLINE -> uint64_t {
-        uint64_t x = v;
+    auto scan = [&](uint32_t v, uint32_t& all) LK_INLINE -> uint32_t {
+        uint32_t x = v;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-            const uint64_t y = __shfl_up(x, d, 64);
+            const uint32_t y = __shfl_up(x, d, 64);
             if ((int)lane >= d) x += y;
         }
         __syncthreads();
         if (lane == 63) s_sum[w] = x;
         __syncthreads();
-        uint64_t before = 0;
+        uint32_t before = 0;
         all = 0;
 #pragma unroll
         for (uint32_t k = 0; k < NW; k++) {
@@ -683,10 +701,9 @@ __device__ __forceinline__ Plan plan_runs(const LkPagedAttn& a, uint32_t wg, uin
         }
         return before + x - v;
     };
-    uint64_t mine = 0, at = 0;
+    uint32_t mine = 0, at = 0;
     for (uint32_t s0 = 0; s0 < a.n; s0 += T) {
-        uint32_t steps;
-        uint64_t all;
+        uint32_t steps, all;
         mine = count(s0 + threadIdx.x, steps);
         at = p.total + scan(mine, all);
         p.total += all;
@@ -703,24 +720,22 @@ __device__ __forceinline__ Plan plan_runs(const LkPagedAttn& a, uint32_t wg, uin
 #pragma unroll
     for (uint32_t k = 0; k < NW; k++) longest = s_long[k] > longest ? s_long[k] : longest;
     // at most kMaxChunks workgroups share an item
-    const uint64_t even = (p.total + gridDim.x - 1) / gridDim.x;
-    const uint32_t few = (longest + kMaxChunks - 3) / (kMaxChunks - 2);
-    const uint64_t run = even > few ? even : few;
-    p.run = (uint32_t)(run > kLeast ? run : kLeast);
+    const uint32_t even = p.total / gridDim.x + 1, few = (longest + kMaxChunks - 3) / (kMaxChunks - 2);
+    p.run = even > few ? even : few;
+    p.run = p.run > kLeast ? p.run : kLeast;
     const uint64_t start = (uint64_t)wg * p.run;
-    uint64_t sum = 0;
+    uint32_t sum = 0;
     for (uint32_t s0 = 0; s0 < a.n; s0 += T) {
         const uint32_t s = s0 + threadIdx.x;
         if (a.n > T) {
-            uint32_t steps;
-            uint64_t all;
+            uint32_t steps, all;
             mine = count(s, steps);
             at = sum + scan(mine, all);
             sum += all;
         }
         if (s < a.n) {
             if (wg == 0) a.place[1 + s] = at;
-            if (start >= at && start < at + mine) s_seq = s, s_at = start - at;
+            if (start >= at && start - at < mine) s_seq = s, s_at = (uint32_t)(start - at);
         }
     }
     if (wg == 0 && threadIdx.x == 0) a.place[0] = p.run;
@@ -751,42 +766,51 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
     constexpr int RING = SIDE * NW <= 8192 * 4 && NW == 4 ? 3 : 2;
     static_assert(OPS >= 1 && SIDE % (1024 * NW) == 0 && 16 % PER == 0, "whole load instructions, each within a tile");
     __shared__ __align__(1024) char ring[RING][2 * SIDE];
+    __shared__ uint32_t s_odd;  // a V that is not finite was met
     typedef __attribute__((address_space(3))) uint32_t* lptr;
     typedef __attribute__((address_space(1))) uint32_t* gptr;
     typedef __attribute__((address_space(3))) s4* sptr;
     const uint32_t lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // neighbours in the order of work are on one XCD (workgroups go round the 8): row groups of a kv head meet in its L2
     const uint32_t wg = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    uint32_t seq;
-    uint64_t in_seq;
-    const Plan plan = plan_runs<NW>(a, wg, STEP, ROWS, seq, in_seq);
-    const uint64_t start = (uint64_t)wg * plan.run;
-    if (start >= plan.total) return;  // uniform
-    const uint64_t left64 = plan.total - start;
-    uint32_t left = left64 < plan.run ? (uint32_t)left64 : plan.run;
-
-    while (left) {
-        Share h{};
-        h.s = seq;
-        h.sq = seq_of<false>(a, seq);
-        const uint32_t groups = row_groups(a, h.sq, ROWS), of_item = groups ? item_steps(h.sq, STEP) : 0;
-        if (in_seq >= (uint64_t)groups * a.p.n_kv * of_item) {  // the sequence is done, or has nothing: on to the next
-            seq++;
-            in_seq = 0;
-            continue;
+    const bool chunks = a.n_chunks != 0;
+    uint32_t seq = 0, in_seq = 0, left = 0;
+    Share h{};
+    if (chunks) {
+        h = share_of<false>(a, ROWS);
+        if (!h.live) return;  // uniform
+    } else {
+        const Plan plan = plan_runs<NW>(a, wg, STEP, ROWS, seq, in_seq);
+        const uint64_t start = (uint64_t)wg * plan.run;
+        if (start >= plan.total) return;  // uniform
+        left = plan.total - start < plan.run ? (uint32_t)(plan.total - start) : plan.run;
+    }
+    do {
+        uint32_t steps;
+        if (chunks) {
+            steps = (h.x1 - h.x0 + STEP - 1) / STEP;
+        } else {
+            h.s = seq;
+            h.sq = seq_of<false>(a, seq);
+            const uint32_t groups = row_groups(a, h.sq, ROWS), of_item = groups ? item_steps(h.sq, STEP) : 0;
+            if (in_seq >= groups * a.p.n_kv * of_item) {  // the sequence is done, or has nothing: on to the next
+                seq++;
+                in_seq = 0;
+                continue;
+            }
+            const uint32_t item = in_seq / of_item, step0 = in_seq - item * of_item;
+            steps = of_item - step0 < left ? of_item - step0 : left;
+            h.kvh = item / groups;
+            h.row0 = (item - h.kvh * groups) * ROWS;
+            h.R = h.sq.rows * a.G;
+            h.x0 = step0 * STEP;
+            h.x1 = (step0 + steps) * STEP < h.sq.total ? (step0 + steps) * STEP : h.sq.total;
+            h.whole = steps == of_item;
+            // a run has at most one part that began before it and one that goes on behind it
+            h.part = ((size_t)wg * 2 + (step0 == 0)) * ROWS;
+            left -= steps;
+            in_seq += steps;
         }
-        const uint32_t item = (uint32_t)(in_seq / of_item), step0 = (uint32_t)(in_seq - (uint64_t)item * of_item);
-        const uint32_t steps = of_item - step0 < left ? of_item - step0 : left;
-        h.kvh = item / groups;
-        h.row0 = (item - h.kvh * groups) * ROWS;
-        h.R = h.sq.rows * a.G;
-        h.x0 = step0 * STEP;
-        h.x1 = (step0 + steps) * STEP < h.sq.total ? (step0 + steps) * STEP : h.sq.total;
-        h.whole = steps == of_item;
-        // a run has at most one part that began before it and one that goes on behind it
-        h.part = ((size_t)wg * 2 + (step0 == 0)) * ROWS;
-        left -= steps;
-        in_seq += steps;
         const uint32_t rbase = h.row0 + w * 32;
         const bool busy = rbase < h.R;  // wave-uniform; an idle wave loads with the others
 
@@ -834,7 +858,8 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
             for (int t = 0; t < NT; t++) b |= tiles >> t & 1 ? 0xFFFFull << (16 * t) : 0;
             return b & low_bits((int64_t)h.sq.total - x);
         };
-        asm volatile("s_barrier" ::: "memory");  // the last part's stages are read
+        __syncthreads();  // the last part's s_odd is read
+        if (threadIdx.x == 0) s_odd = 0;  // set behind a barrier at the earliest
         uint32_t tiles[RING - 1];  // of the steps under way: which tiles are no holes
 #pragma unroll
         for (int n = 0; n < RING - 1; n++) {
@@ -882,7 +907,6 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
             const uint32_t x = h.x0 + n * STEP;
             const bool masked = tl != (1u << NT) - 1 || x + STEP > h.sq.ctx;  // uniform: something to hide
             uint64_t live = 0;
-            bool odd = false;
             if (masked) {
                 // V of positions that no row sees becomes zero, and what is not finite too
                 live = live_of(x, tl);
@@ -895,22 +919,23 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
                     for (int e = 0; e < 4; e++) y[e] = Wave::clean_word(see ? y[e] : 0, any);
                     *at = y;
                 }
-                odd = __syncthreads_or(any != 0);
+                if (any) s_odd = 1;
+                __syncthreads();
             }
             if (!busy) continue;
             f4 sc[RT][NT];
-            {
-                u4 kr[NT][KS];
+            r.start(sc);
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++)
+            for (int ks = 0; ks < KS; ks++) {
+                u4 kr[NT];
 #pragma unroll
-                    for (int t = 0; t < NT; t++) kr[t][ks] = *(const u4*)(stage + k_at[ks] + t * 16 * RB);
-                r.scores(kr, sc);
+                for (int t = 0; t < NT; t++) kr[t] = *(const u4*)(stage + k_at[ks] + t * 16 * RB);
+                r.scores(kr, ks, sc);
+                if (HD == 128 && ks % 2) __builtin_amdgcn_sched_barrier(0);  // K operands of two at a time: registers
             }
             if (masked) {
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt), sc);
-                if (odd) r.poison(a, h, x, live);
             }
             r.move(sc, scaled);
             if constexpr (F32) {
@@ -926,23 +951,33 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
                             for (int e = 0; e < 4; e++) y[d + e] = z[e];
                         }
                         r.add32(sc, t, i, y);
+                        if (HD == 128 && i % 2) __builtin_amdgcn_sched_barrier(0);
                     }
             } else {
 #pragma unroll
                 for (int g = 0; g < NT / 2; g++) {
-                    h8 vb[ND];
+                    h8 ph[RT], pl[RT];
+                    r.weights(sc, g, ph, pl);
 #pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        u2 y[2];
+                    for (int d0 = 0; d0 < ND; d0 += 4) {
+                        h8 vb[4];
 #pragma unroll
-                        for (int t = 0; t < 2; t++)
-                            y[t] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((sptr)(stage + v_at[d][0] + (2 * g + t) * 16 * RB)));
-                        vb[d] = __builtin_bit_cast(h8, u4{y[0][0], y[0][1], y[1][0], y[1][1]});
+                        for (int d = 0; d < 4; d++) {
+                            u2 y[2];
+#pragma unroll
+                            for (int t = 0; t < 2; t++)
+                                y[t] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((sptr)(stage + v_at[d0 + d][0] + (2 * g + t) * 16 * RB)));
+                            vb[d] = __builtin_bit_cast(h8, u4{y[0][0], y[0][1], y[1][0], y[1][1]});
+                        }
+                        r.add16(ph, pl, vb, d0);
+                        if (HD == 128) __builtin_amdgcn_sched_barrier(0);
                     }
-                    r.add16(sc, g, vb);
                 }
             }
         }
+        __syncthreads();  // s_odd, and the stages, are settled
+        if (s_odd && busy)
+            for (uint32_t n = 0; n < steps; n++) r.poison(a, h, h.x0 + n * STEP);
         if (!busy) continue;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
@@ -954,14 +989,14 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
                 const float top = r.max_of(rt, i), sum = r.sum_of(rt, i);
                 r.put(a, h, w * 32 + rt * 16 + 4 * r.j + i, top, sum, y);
             }
-    }
+    } while (left);
 }
 
 // Parts of a row, joined.  A block takes four rows: a wave weighs a row's parts (lane = part, at most 64), then HD / 4
 // lanes by SPLIT groups a row add them up, each group every SPLIT-th part: two dependent reads of memory in all.  (One
 // thread group walking the parts of a row: 19.6 us for 33 parts of 112 rows x 8.)  ROWS: of a workgroup of the wide
 // kernel; 0: parts are the narrow kernel's chunks.
-template <int HD, bool SPARSE, int ROWS, int STEP>
+template <int HD, bool SPARSE, int ROWS, uint32_t STEP>
 __global__ __launch_bounds__(256) void paged_fold_kernel(const LkPagedAttn a) {
     constexpr uint32_t L = HD / 4, SPLIT = 64 / L;
     __shared__ float s_f[4][kMaxChunks];
@@ -970,22 +1005,24 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const LkPagedAttn a) {
     const Seq sq = seq_of<SPARSE>(a, s);
     const uint32_t R = sq.rows * a.G, w = threadIdx.x >> 6, lane = threadIdx.x & 63, row = blockIdx.y * 4 + w;
     if (!sq.live || blockIdx.y * 4 >= R) return;  // uniform
+    constexpr uint32_t RG = ROWS ? ROWS : 1;
     uint32_t parts;
-    size_t base, stride;  // of the row's parts, but for the wide kernel's first
-    if constexpr (ROWS) {
-        const uint32_t groups = row_groups(a, sq, ROWS), of_item = item_steps(sq, STEP), run = (uint32_t)a.place[0];
-        const uint64_t at = a.place[1 + s] + (uint64_t)(kvh * groups + blockIdx.y * 4 / ROWS) * of_item;
+    size_t base, stride;  // of the row's parts, but for the first of runs
+    const bool runs = ROWS && !a.n_chunks;
+    if (runs) {
+        const uint32_t groups = row_groups(a, sq, RG), of_item = item_steps(sq, STEP), run = (uint32_t)a.place[0];
+        const uint64_t at = a.place[1 + s] + (uint64_t)(kvh * groups + blockIdx.y * 4 / RG) * of_item;
         const uint64_t wg = at / run;
         parts = (uint32_t)((at + of_item - 1) / run - wg) + 1;
-        base = wg * 2 * ROWS + row % ROWS;
-        stride = 2 * ROWS;
+        base = wg * 2 * RG + row % RG;
+        stride = 2 * RG;
     } else {
         parts = chunks_of(sq.total, a.chunk);
         base = (size_t)pair * a.n_chunks * a.rows_pad + row;
         stride = a.rows_pad;
     }
     if (parts == 1) return;  // uniform: written as it is
-    auto at = [&](uint32_t k) LK_INLINE { return base + k * stride + (ROWS && k == 0 ? ROWS : 0); };
+    auto at = [&](uint32_t k) LK_INLINE { return base + k * stride + (runs && k == 0 ? RG : 0); };
     if (row < R) {  // wave-uniform
         float2 ml{-INFINITY, 0.f};
         if (lane < parts) ml = *(const float2*)(a.part_ml + 2 * at(lane));
@@ -1025,27 +1062,32 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
     p.rows_pad = p.n_rg * per;
     const uint64_t base = (uint64_t)n * n_kv * p.n_rg;
     const uint32_t step = f32 || hd == 128 ? 32 : 64;
-    if (p.narrow) {
-        const uint32_t all = step * 4;  // every wave has a step
-        const uint64_t steps = (positions + all - 1) / all;
-        uint64_t c = (1024 + base - 1) / base;
+    const uint64_t steps = (positions + step - 1) / step, fill = (uint64_t)kCus * LK_WIDE_OCC * 4 / p.waves;
+    p.steps = base * steps;
+    if (!p.narrow && p.steps > (f32 ? 4 : 16) * fill) {
+        p.blocks = fill;
+        p.part_rows = fill * 2 * per;
+        p.place_bytes = (((uint64_t)n + 1) * 8 + 255) / 256 * 256;
+    } else {
+        const uint32_t all = p.narrow ? step * 4 : step;  // narrow: every wave has a step
+        const uint64_t pieces = (positions + all - 1) / all;
+        uint64_t c;
+        if (p.narrow) {
+            c = (1024 + base - 1) / base;
+        } else {  // chunks of 512 positions, shorter ones if that leaves too few
+            const uint64_t by_len = (positions + 511) / 512, by_fill = (512 + base - 1) / base;
+            c = by_len > by_fill ? by_len : by_fill;
+        }
         c = c > kMaxChunks ? kMaxChunks : c;
-        c = c > steps ? steps : c;
+        c = c > pieces ? pieces : c;
         if (c < 1) c = 1;
-        p.chunk = (uint32_t)((steps + c - 1) / c * all);
+        p.chunk = (uint32_t)((pieces + c - 1) / c * all);
         if (!p.chunk) p.chunk = all;
         p.n_chunks = (uint32_t)((positions + p.chunk - 1) / p.chunk);
         if (!p.n_chunks) p.n_chunks = 1;
         const uint64_t items = (uint64_t)n * n_kv * p.n_chunks;
         p.blocks = (items + 7) / 8 * 8 * p.n_rg;
         p.part_rows = p.n_chunks > 1 ? items * p.rows_pad : 0;
-    } else {
-        const uint64_t steps = base * ((positions + step - 1) / step), most = (steps + kLeast - 1) / kLeast;
-        const uint64_t fill = (uint64_t)kCus * LK_WIDE_OCC * 4 / p.waves;
-        p.blocks = ((fill < most ? fill : most) + 7) / 8 * 8;
-        p.part_rows = p.blocks * 2 * per;
-        p.place_bytes = ((uint64_t)n + 1) * 8;
-        p.place_bytes = (p.place_bytes + 255) / 256 * 256;
     }
     p.part_bytes = p.place_bytes + p.part_rows * (hd + 2) * 4;
     return p;
@@ -1065,7 +1107,7 @@ static hipError_t launch(const LkPagedAttn& a, const LkPagedPlan& p, hipStream_t
 #define LK_WIDE(NW)                                                                                                   \
     hipLaunchKernelGGL((paged_wide_kernel<HD, F32, NW>), grid, dim3(NW * 64), 0, st, a);                              \
     const hipError_t e = hipGetLastError();                                                                           \
-    if (e != hipSuccess) return e;                                                                                    \
+    if (e != hipSuccess || p.n_chunks == 1) return e;                                                                 \
     hipLaunchKernelGGL((paged_fold_kernel<HD, false, Wide<HD, F32, NW>::ROWS, Wide<HD, F32, NW>::STEP>), fold,        \
                        dim3(256), 0, st, a)
         if (p.waves == 2) {

@@ -70,7 +70,7 @@ struct LkPagedPlan {
     bool narrow;           // waves take positions in turn; else they lie side by side in rows
     uint32_t tiles, waves; // 16-row tiles of a wave, waves of a workgroup
     uint32_t chunk, n_chunks, n_rg, rows_pad;
-    uint64_t blocks;
+    uint64_t blocks, steps;  // steps: of all items at the table's capacity
     uint64_t place_bytes, part_rows, part_bytes;
 };
 // positions: the most that a sequence can show (its table's capacity; sparse: take pages)

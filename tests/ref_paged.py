@@ -133,9 +133,9 @@ def choose(c, s, q, ctx, bounds, heads, take, first, last):
                 continue
             b = bounds[i, h].astype(np.float64)
             qq = q[h * G * c.hd:(h + 1) * G * c.hd].reshape(G, c.hd).astype(np.float64)
-            score[x] = (qq * np.where(qq > 0, b[1], b[0])).sum(1).max()
+            score[x] = (qq * np.where(qq > 0, b[1], b[0])).sum(1).max() if np.isfinite(b).all() else np.nan
         keep = [x for x in range(held) if x < first or x >= held - last]
-        # NaN first, then by score, then the lowest page
+        # bounds that are not finite first, then by score, then the lowest page
         rest = sorted((x for x in range(held) if x not in keep),
                       key=lambda x: (not np.isnan(score[x]), 0 if np.isnan(score[x]) else -score[x], x))
         out[h, :take] = sorted(keep + rest[:take - len(keep)])
