@@ -97,6 +97,21 @@ __device__ __forceinline__ float lk_wave_max(float v) {
     v = fmaxf(v, lk_dpp<0x143, 0xC>(v, ninf));
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
+// Inclusive sum over the wave's lanes up to this one: row_shr 1, 2, 4, 8 within rows of 16 (lanes without a source add
+// 0), then the row totals by row_bcast 15 and 31.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t lk_dpp_u32(uint32_t v, uint32_t old) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROW_MASK, 0xF, false);
+}
+__device__ __forceinline__ uint32_t lk_wave_scan(uint32_t v) {
+    v += lk_dpp_u32<0x111, 0xF>(v, 0);
+    v += lk_dpp_u32<0x112, 0xF>(v, 0);
+    v += lk_dpp_u32<0x114, 0xF>(v, 0);
+    v += lk_dpp_u32<0x118, 0xF>(v, 0);
+    v += lk_dpp_u32<0x142, 0xA>(v, 0);
+    v += lk_dpp_u32<0x143, 0xC>(v, 0);
+    return v;
+}
 // Sum over the four lanes {l, l^8, l^16 .. within one 32-lane half}: row_ror 8
 // then an xor-16 swizzle.  Lane l of each half then holds the sum of the four
 // lanes of that half with the same (l & 7).

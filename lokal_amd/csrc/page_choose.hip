@@ -17,9 +17,9 @@ __device__ __forceinline__ uint64_t order_key(double x) {
 // score(page) = max over the kv head's query heads of sum_d max(q_d lo_d, q_d hi_d),
 // which no q.k of the page exceeds; products of f32 and f16 are exact in 64 bits and
 // their sums wrong by 2^-52, so that which page is taken does not hang on the order of
-// a sum (f64 products run at the f32 rate here).  Eight lanes take a page, E = HD / 8
-// dims each, as max(q, 0) hi + min(q, 0) lo: two products a dim and head, the bounds
-// widened once for all heads.  A bound that is not finite makes the sum so too.
+// a sum (f64 products run at the f32 rate here).  HD / 8 lanes take a page, E = 8
+// dims each; the bounds are widened once for all heads, and the sign of q_d says which
+// one a dim needs.  A page with a bound that is not finite has the highest key.
 template <int N>
 __device__ __forceinline__ double dpp_add(double x) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
@@ -27,12 +27,16 @@ __device__ __forceinline__ double dpp_add(double x) {
     const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), N, 0xF, 0xF, false);
     return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-// over eight neighbouring lanes: quad pairs, quad halves, the half row mirrored
-__device__ __forceinline__ double sum8(double x) { return dpp_add<0x141>(dpp_add<0x4E>(dpp_add<0xB1>(x))); }
+// over N = 8 or 16 neighbouring lanes: quad pairs, quad halves, the half row mirrored, the row mirrored
+template <int N>
+__device__ __forceinline__ double lanes_sum(double x) {
+    x = dpp_add<0x141>(dpp_add<0x4E>(dpp_add<0xB1>(x)));
+    return N == 16 ? dpp_add<0x140>(x) : x;
+}
 
 template <typename KV, int HD>
 struct PageBounds {
-    static constexpr int E = HD / 8, W = E * sizeof(KV) / 4;  // words of a lane's lower, and of its upper bounds
+    static constexpr int E = 8, W = E * sizeof(KV) / 4;  // words of a lane's lower, and of its upper bounds
     uint32_t lo[W], hi[W];
     __device__ __forceinline__ void load(const void* bounds, const LkPages& p, uint32_t id, uint32_t kvh, uint32_t c) {
         const u4* b = (const u4*)((const KV*)bounds + ((size_t)id * p.n_kv + kvh) * 2 * HD + c * E);
@@ -45,15 +49,30 @@ struct PageBounds {
         }
     }
     // The bounds of dim e of the lane.
-    __device__ __forceinline__ double low(int e) const {
-        if constexpr (sizeof(KV) == 4) return (double)__uint_as_float(lo[e]);
-        else return (double)lk_h2f((uint16_t)(lo[e / 2] >> (16 * (e & 1))));
+    __device__ __forceinline__ float low(int e) const {
+        if constexpr (sizeof(KV) == 4) return __uint_as_float(lo[e]);
+        else return lk_h2f((uint16_t)(lo[e / 2] >> (16 * (e & 1))));
     }
-    __device__ __forceinline__ double high(int e) const {
-        if constexpr (sizeof(KV) == 4) return (double)__uint_as_float(hi[e]);
-        else return (double)lk_h2f((uint16_t)(hi[e / 2] >> (16 * (e & 1))));
+    __device__ __forceinline__ float high(int e) const {
+        if constexpr (sizeof(KV) == 4) return __uint_as_float(hi[e]);
+        else return lk_h2f((uint16_t)(hi[e / 2] >> (16 * (e & 1))));
     }
 };
+
+// AND and OR over the wave, on lane 63: as a sum by lk_wave_sum's steps (a lane without a source meets itself).
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint64_t dpp_bits(uint64_t x) {
+    const uint32_t lo = (uint32_t)x, hi = (uint32_t)(x >> 32);
+    return (uint64_t)lk_dpp_u32<CTRL, ROW_MASK>(hi, hi) << 32 | lk_dpp_u32<CTRL, ROW_MASK>(lo, lo);
+}
+__device__ __forceinline__ void wave_bits(uint64_t& all, uint64_t& any) {
+    all &= dpp_bits<0xB1, 0xF>(all), any |= dpp_bits<0xB1, 0xF>(any);
+    all &= dpp_bits<0x4E, 0xF>(all), any |= dpp_bits<0x4E, 0xF>(any);
+    all &= dpp_bits<0x124, 0xF>(all), any |= dpp_bits<0x124, 0xF>(any);
+    all &= dpp_bits<0x128, 0xF>(all), any |= dpp_bits<0x128, 0xF>(any);
+    all &= dpp_bits<0x142, 0xA>(all), any |= dpp_bits<0x142, 0xA>(any);
+    all &= dpp_bits<0x143, 0xC>(all), any |= dpp_bits<0x143, 0xC>(any);
+}
 
 // What a sequence holds, for both kernels below.
 __device__ __forceinline__ uint32_t sparse_held(const LkSparse& a, uint32_t slot, uint32_t s) {
@@ -65,41 +84,60 @@ __device__ __forceinline__ bool sparse_forced(const LkSparse& a, uint32_t x, uin
     return x < a.first || x + a.last >= held;
 }
 
-// Keys of pages x0, x0 + step, .. below x1 for one (sequence, kv head), by groups of 8
+// Keys of pages x0, x0 + step, .. below x1 for one (sequence, kv head), by groups of HD / 8
 // lanes; put(page, key) runs on one lane of the group.  s_q: kHeads x HD doubles.
 constexpr uint32_t kHeads = 8;
 template <typename KV, int HD, class Put>
 __device__ __forceinline__ void score_pages(const LkSparse& a, uint32_t s, uint32_t slot, uint32_t kvh, uint32_t held,
                                             uint32_t x0, uint32_t x1, uint32_t step, double* s_q, Put put) {
-    constexpr int E = HD / 8;
-    const uint32_t c = threadIdx.x & 7;
+    constexpr int E = 8, L = HD / 8;
+    const uint32_t c = threadIdx.x % L;
     const uint32_t* row = a.t.table + (size_t)slot * a.t.max_pages;
+    // a page's id is read two pages ahead, its bounds one
+    auto id_of = [&](uint32_t x) __attribute__((always_inline)) -> uint32_t {
+        return x < x1 && !sparse_forced(a, x, held) ? row[x] : LK_NO_PAGE;
+    };
     for (uint32_t g0 = 0; g0 < a.G; g0 += kHeads) {
+        uint32_t id = id_of(x0), id1 = id_of(x0 + step);
+        PageBounds<KV, HD> b;
+        b.load(a.bounds, a.p, id < a.p.n_pages ? id : 0, kvh, c);
         const uint32_t gn = a.G - g0 < kHeads ? a.G - g0 : kHeads;
         __syncthreads();  // the last heads' q is read
         const float* q = a.q + ((size_t)s * a.n_heads + kvh * a.G + g0) * HD;
-        for (uint32_t i = threadIdx.x; i < gn * HD; i += blockDim.x) s_q[i] = q[i];
+        // [head][pair of a lane's dims][lane][2]: neighbouring lanes read neighbouring 16 bytes
+        for (uint32_t i = threadIdx.x; i < gn * HD; i += blockDim.x)
+            s_q[i / HD * HD + (i % E / 2 * L + i % HD / E) * 2 + i % 2] = q[i];
         __syncthreads();
         for (uint32_t x = x0; x < x1; x += step) {
+            const PageBounds<KV, HD> now = b;
+            const bool there = id < a.p.n_pages;
+            id = id1;
+            b.load(a.bounds, a.p, id < a.p.n_pages ? id : 0, kvh, c);
+            id1 = id_of(x + 2 * step);
             if (sparse_forced(a, x, held)) continue;
-            const uint32_t id = row[x];
             uint64_t key = 0;  // a hole: below all
-            if (id < a.p.n_pages) {
-                PageBounds<KV, HD> b;
-                b.load(a.bounds, a.p, id, kvh, c);
+            if (there) {
                 double bl[E], bh[E];
+                float odd = 0.f;  // NaN where a bound is not finite
 #pragma unroll
-                for (int e = 0; e < E; e++) bl[e] = b.low(e), bh[e] = b.high(e);
+                for (int e = 0; e < E; e++) {
+                    const float u = now.low(e), v = now.high(e);
+                    odd = fmaf(v, 0.f, fmaf(u, 0.f, odd));
+                    bl[e] = u, bh[e] = v;
+                }
+                double top = -(double)INFINITY, off = odd;
                 for (uint32_t g = 0; g < gn; g++) {
-                    double sum = 0;
+                    double sum = off;
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        const double y = s_q[g * HD + c * E + e];
-                        sum = fma(fmax(y, 0.0), bh[e], fma(fmin(y, 0.0), bl[e], sum));
+                        const double y = s_q[g * HD + (e / 2 * L + c) * 2 + e % 2];
+                        sum = fma(y, __double2hiint(y) < 0 ? bl[e] : bh[e], sum);
                     }
-                    const uint64_t k = order_key(sum8(sum));
-                    key = k > key ? k : key;
+                    sum = lanes_sum<L>(sum);
+                    top = sum > top || !(fabs(sum) < (double)INFINITY) ? sum : top;
+                    off = fabs(sum) < (double)INFINITY ? off : (double)NAN;  // and stays so
                 }
+                key = order_key(top);
             }
             if (c == 0) put(x, key, g0 == 0);
         }
@@ -114,7 +152,7 @@ __global__ __launch_bounds__(256) void sparse_score_kernel(const LkSparse a) {
     const uint32_t held = sparse_held(a, slot, s);
     if (held <= a.take) return;  // uniform: all are taken
     uint64_t* keys = a.keys + ((size_t)s * a.p.n_kv + kvh) * a.t.max_pages;
-    score_pages<KV, HD>(a, s, slot, kvh, held, blockIdx.x * 32 + threadIdx.x / 8, held, gridDim.x * 32, s_q,
+    score_pages<KV, HD>(a, s, slot, kvh, held, blockIdx.x * (2048 / HD) + threadIdx.x / (HD / 8), held, gridDim.x * (2048 / HD), s_q,
                         [&](uint32_t x, uint64_t k, bool first) { keys[x] = first || k > keys[x] ? k : keys[x]; });
 }
 
@@ -123,10 +161,7 @@ __global__ __launch_bounds__(256) void sparse_score_kernel(const LkSparse a) {
 // pages above it and the first of those at it, in order: equal keys go to the lowest
 // page.  One workgroup a (sequence, kv head); FUSED: it takes the scores itself and
 // keeps the keys in LDS.  (A thread that walks 256 bins eight times: 62-78 us.)
-#ifndef LK_FUSED_PAGES
-#define LK_FUSED_PAGES 256
-#endif
-constexpr uint32_t kBins = 2048, kFusedPages = LK_FUSED_PAGES;
+constexpr uint32_t kBins = 2048, kFusedPages = 256;
 template <typename KV, int HD, bool FUSED, uint32_t kChoose>
 __global__ __launch_bounds__(kChoose) void sparse_choose_kernel(const LkSparse a) {
     __shared__ uint32_t s_bin[kBins], s_part[kChoose / 64], s_find[3];
@@ -143,7 +178,7 @@ __global__ __launch_bounds__(kChoose) void sparse_choose_kernel(const LkSparse a
     }
     const uint64_t* keys;
     if constexpr (FUSED) {
-        score_pages<KV, HD>(a, s, slot, kvh, held, tid / 8, held, kChoose / 8, s_q,
+        score_pages<KV, HD>(a, s, slot, kvh, held, tid / (HD / 8), held, kChoose / (HD / 8), s_q,
                             [&](uint32_t x, uint64_t k, bool first) { s_keys[x] = first || k > s_keys[x] ? k : s_keys[x]; });
         keys = s_keys;
         __syncthreads();
@@ -152,12 +187,7 @@ __global__ __launch_bounds__(kChoose) void sparse_choose_kernel(const LkSparse a
     }
     // sum of v over the threads before this one, and over all
     auto scan = [&](uint32_t v, uint32_t& all) {
-        uint32_t x = v;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t y = __shfl_up(x, d, 64);
-            if ((int)lane >= d) x += y;
-        }
+        const uint32_t x = lk_wave_scan(v);
         __syncthreads();
         if (lane == 63) s_part[w] = x;
         __syncthreads();
@@ -182,14 +212,14 @@ __global__ __launch_bounds__(kChoose) void sparse_choose_kernel(const LkSparse a
             const uint64_t k = keys[x];
             if (asked(x, k)) all1 &= k, any1 |= k;
         }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) all1 &= __shfl_xor(all1, d, 64), any1 |= __shfl_xor(any1, d, 64);
+        wave_bits(all1, any1);
         __syncthreads();
-        if (lane == 0) s_and[w] = all1, s_or[w] = any1;
+        if (lane == 63) s_and[w] = all1, s_or[w] = any1;
         for (uint32_t b = tid; b < kBins; b += kChoose) s_bin[b] = 0;
         __syncthreads();
+        all1 = s_and[0], any1 = s_or[0];
 #pragma unroll
-        for (uint32_t k = 0; k < kChoose / 64; k++) all1 &= s_and[k], any1 |= s_or[k];
+        for (uint32_t k = 1; k < kChoose / 64; k++) all1 &= s_and[k], any1 |= s_or[k];
         const uint64_t differ = all1 ^ any1;
         if (!differ) {  // all in question are equal
             shift = 0;
@@ -258,8 +288,8 @@ static void select_launch(const LkSparse& a, hipStream_t st) {
         hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, true, 256>), pairs, dim3(256), 0, st, a);
         return;
     }
-    uint32_t blocks = 2048 / (a.n * a.p.n_kv) + 1;
-    const uint32_t most = (a.t.max_pages + 31) / 32;
+    uint32_t blocks = 4096 / (a.n * a.p.n_kv) + 1;
+    const uint32_t most = (a.t.max_pages + 2048 / HD - 1) / (2048 / HD);
     if (blocks > most) blocks = most;
     hipLaunchKernelGGL((sparse_score_kernel<KV, HD>), dim3(blocks, a.p.n_kv, a.n), dim3(256), 0, st, a);
     if (a.t.max_pages <= 2048) hipLaunchKernelGGL((sparse_choose_kernel<KV, HD, false, 256>), pairs, dim3(256), 0, st, a);

@@ -23,8 +23,7 @@
 // so most steps neither reduce over lanes nor rescale O; P stays below 2^8.
 //
 // Two kernels.  Up to 32 rows (narrow): the four waves of a workgroup take steps in
-// turn, K and V go straight from memory to registers, the next step's while this
-// one's are used, and the waves join at the end.  More rows (wide): the waves lie
+// turn, K and V go straight from memory to registers, and the waves join at the end.  More rows (wide): the waves lie
 // side by side in rows and share each step's K and V through LDS, a ring of stages
 // that loads write without registers.
 //
@@ -485,7 +484,7 @@ struct Rows {
 // ---------------------------------------------------------------- narrow
 
 template <int HD, bool F32, int RT, bool SPARSE>
-__global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) {
+__global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow_kernel(const LkPagedAttn a) {
     constexpr int NT = F32 || HD == 128 ? 2 : 4, W = 4, ROWS = RT * 16, STEP = NT * 16;
     using Wave = Rows<HD, F32, RT, NT, SPARSE, false>;
     constexpr int ND = Wave::ND, KS = Wave::KS, VW = Wave::VW, ES = Wave::ES;
@@ -495,9 +494,6 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
     if (!h.live) return;  // uniform
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Wave r;
-    bool scaled;
-    u4 kr[2][NT][KS];
-    uint32_t vr[2][NT][4][VW];
     // a step's tiles: loads go out for all of its K and V
     auto fetch = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t& live, bool& masked) LK_INLINE {
         const uint32_t j = (threadIdx.x & 63) >> 4, c16 = threadIdx.x & 15;
@@ -540,7 +536,7 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
             }
     };
     uint32_t odd = 0;
-    auto use = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t live, bool masked) LK_INLINE {
+    auto use = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t live, bool masked, bool scaled) LK_INLINE {
         f4 sc[RT][NT];
         r.start(sc);
 #pragma unroll
@@ -583,21 +579,15 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(const LkPagedAttn a) 
             }
         }
     };
+    const bool scaled = r.init(a, h, h.row0);
     uint32_t x = h.x0 + w * STEP;
-    uint64_t live[2];
-    bool masked[2];
-    if (x < h.x1) fetch(x, kr[0], vr[0], live[0], masked[0]);
-    scaled = r.init(a, h, h.row0);
-    while (x < h.x1) {
-        uint32_t nx = x + W * STEP;
-        if (nx < h.x1) fetch(nx, kr[1], vr[1], live[1], masked[1]);
-        use(x, kr[0], vr[0], live[0], masked[0]);
-        x = nx;
-        if (x >= h.x1) break;
-        nx = x + W * STEP;
-        if (nx < h.x1) fetch(nx, kr[0], vr[0], live[0], masked[0]);
-        use(x, kr[1], vr[1], live[1], masked[1]);
-        x = nx;
+    for (; x < h.x1; x += W * STEP) {
+        u4 k[NT][KS];
+        uint32_t v[NT][4][VW];
+        uint64_t live;
+        bool masked;
+        fetch(x, k, v, live, masked);
+        use(x, k, v, live, masked, scaled);
     }
     if (!SPARSE && __any(odd))
         for (x = h.x0 + w * STEP; x < h.x1; x += W * STEP) r.poison(a, h, x);

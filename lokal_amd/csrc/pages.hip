@@ -73,29 +73,18 @@ __global__ __launch_bounds__(256) void pages_trim_kernel(LkPages p, LkTable t, c
 
 // ------------------------------------------------------------------ grow
 
-constexpr uint32_t kGrowThreads = 1024;
-constexpr uint32_t kScan = 4;  // refs a thread looks at in one go
+constexpr uint32_t kScan = 4;
 
 // Exclusive sum of v over the block's threads, and the total.  part: one word per wave.
-template <typename T>
-__device__ __forceinline__ T block_exclusive(T v, T* part, T& total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-    T x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const T y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* part, uint32_t& total) {
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, x = lk_wave_scan(v);
     __syncthreads();  // part is free
     if (lane == 63) part[w] = x;
     __syncthreads();
-    T before = 0;
-    total = 0;
-    for (int k = 0; k < nw; k++) {
-        if (k < w) before += part[k];
-        total += part[k];
-    }
-    return before + x - v;
+    // the waves before this one: a lane each
+    const uint32_t y = lk_wave_scan(lane < nw ? part[lane] : 0);
+    total = __builtin_amdgcn_readlane(y, 63);
+    return (w ? __builtin_amdgcn_readlane(y, w - 1) : 0) + x - v;
 }
 
 // One workgroup, entry i on thread i: what each entry needs, an exclusive sum
@@ -103,24 +92,25 @@ __device__ __forceinline__ T block_exclusive(T v, T* part, T& total) {
 // that owns rank r.  An entry is refused (and changes nothing) where its row
 // does not exist, came before, has no room, or where the free pages end
 // before its last one; entries that need none are never refused for that.
-__global__ __launch_bounds__(kGrowThreads) void pages_grow_kernel(LkPages p, LkTable t, const uint32_t* slots,
-                                                                  const uint32_t* add, uint32_t n, uint32_t* ok,
-                                                                  uint32_t* copied) {
-    __shared__ uint32_t s_slot[LK_PAGES_LIST_MAX], s_first[LK_PAGES_LIST_MAX], s_to[LK_PAGES_LIST_MAX];
-    __shared__ uint64_t s_off[LK_PAGES_LIST_MAX + 1], s_part64[kGrowThreads / 64];
-    __shared__ uint32_t s_part[kGrowThreads / 64];
+// T: threads, at least n; kScan refs a thread looks at in one go.
+template <uint32_t T>
+__global__ __launch_bounds__(T) void pages_grow_kernel(LkPages p, LkTable t, const uint32_t* slots,
+                                                       const uint32_t* add, uint32_t n, uint32_t* ok,
+                                                       uint32_t* copied) {
+    __shared__ uint32_t s_slot[T], s_first[T], s_to[T], s_off[T], s_part[T / 64], s_end[T / 64];
     const uint32_t i = threadIdx.x;
     const uint32_t page = 1u << p.pshift;
     const uint32_t slot = i < n ? slots[i] : LK_NO_PAGE;
+    const uint32_t more = i < n ? add[i] : 0;
     s_slot[i] = slot;
     s_to[i] = LK_NO_PAGE;
     __syncthreads();
     bool valid = slot < t.n_seq;
     for (uint32_t j = 0; j < i && valid; j++) valid = s_slot[j] != slot;
-    uint32_t old = LK_NO_PAGE;
-    uint64_t need = 0, now = 0;
+    uint32_t old = LK_NO_PAGE, need = 0;
+    uint64_t now = 0;
     if (valid) {
-        const uint32_t len = t.len[slot], more = add[i];
+        const uint32_t len = t.len[slot];
         now = (uint64_t)len + more;
         const uint64_t want = (now + page - 1) >> p.pshift;
         const uint32_t held = pages_of(len, p.pshift);
@@ -132,65 +122,66 @@ __global__ __launch_bounds__(kGrowThreads) void pages_grow_kernel(LkPages p, LkT
             }
             const uint32_t first = held - (old != LK_NO_PAGE);
             s_first[i] = first;
-            need = want > first ? want - first : 0;
+            need = want > first ? (uint32_t)want - first : 0;
         }
     }
-    uint64_t total;
-    const uint64_t off = block_exclusive(need, s_part64, total);
+    // The sum in two halves of 32 bits, as a need is below 2^27 + 1; what passes 32 bits together is more than there can
+    // be free.
+    uint32_t total_lo, total_hi;
+    const uint32_t off_lo = block_exclusive(need & 0xFFFF, s_part, total_lo), off_hi = block_exclusive(need >> 16, s_part, total_hi);
+    auto whole = [](uint32_t hi, uint32_t lo) {
+        const uint64_t x = ((uint64_t)hi << 16) + lo;
+        return x < 0xFFFFFFFFull ? (uint32_t)x : 0xFFFFFFFFu;
+    };
+    const uint32_t off = whole(off_hi, off_lo), total = whole(total_hi, total_lo);
     s_off[i] = off;
-    if (i == kGrowThreads - 1) s_off[kGrowThreads] = total;
     // how many of the `total` pages there are
-    uint64_t n_free = 0;
-    for (uint64_t x0 = 0; x0 < p.n_pages && n_free < total; x0 += kGrowThreads * kScan) {
+    uint32_t n_free = 0;
+    for (uint32_t x0 = 0; x0 < p.n_pages && n_free < total; x0 += T * kScan) {  // below 2^31 + T * kScan
         uint32_t c = 0, all;
 #pragma unroll
         for (uint32_t k = 0; k < kScan; k++) {
-            const uint64_t x = x0 + i * kScan + k;
+            const uint32_t x = x0 + i * kScan + k;
             c += x < p.n_pages && t.refs[x] == 0;
         }
         (void)block_exclusive(c, s_part, all);
         n_free += all;
     }
-    const bool grows = valid && (need == 0 || off + need <= n_free);
+    const bool grows = valid && (need == 0 || (uint64_t)off + need <= n_free);
     // the ranks that are given out end with the last entry that takes any
-    __syncthreads();
-    uint64_t end = 0;
-    {
-        const uint64_t mine = grows && need ? off + need : 0;
-        uint64_t m = mine;
+    uint32_t end = grows && need ? off + need : 0;
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint64_t y = __shfl_xor(m, d, 64);
-            m = y > m ? y : m;
-        }
-        if ((i & 63) == 0) s_part64[i >> 6] = m;
-        __syncthreads();
-        for (uint32_t k = 0; k < kGrowThreads / 64; k++) end = s_part64[k] > end ? s_part64[k] : end;
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t y = __shfl_xor(end, d, 64);
+        end = y > end ? y : end;
     }
-    uint64_t rank = 0;
-    for (uint64_t x0 = 0; x0 < p.n_pages && rank < end; x0 += kGrowThreads * kScan) {
+    if ((i & 63) == 0) s_end[i >> 6] = end;
+    __syncthreads();
+    for (uint32_t k = 0; k < T / 64; k++) end = s_end[k] > end ? s_end[k] : end;
+    uint32_t rank = 0;
+    for (uint32_t x0 = 0; x0 < p.n_pages && rank < end; x0 += T * kScan) {
         uint32_t c = 0, all;
         bool is_free[kScan];
 #pragma unroll
         for (uint32_t k = 0; k < kScan; k++) {
-            const uint64_t x = x0 + i * kScan + k;
+            const uint32_t x = x0 + i * kScan + k;
             is_free[k] = x < p.n_pages && t.refs[x] == 0;
             c += is_free[k];
         }
-        uint64_t r = rank + block_exclusive(c, s_part, all);
+        uint32_t r = rank + block_exclusive(c, s_part, all);
 #pragma unroll
         for (uint32_t k = 0; k < kScan; k++) {
             if (!is_free[k]) continue;
             if (r < end) {
                 // the entry e with off[e] <= r < off[e + 1]: the last one with off <= r, as entries that need none share
                 // their offset with the one behind them
-                uint32_t lo = 0, hi = kGrowThreads;
+                uint32_t lo = 0, hi = T;
                 while (hi - lo > 1) {
                     const uint32_t mid = (lo + hi) / 2;
                     if (s_off[mid] <= r) lo = mid;
                     else hi = mid;
                 }
-                const uint32_t id = (uint32_t)(x0 + i * kScan + k), k0 = (uint32_t)(r - s_off[lo]);
+                const uint32_t id = x0 + i * kScan + k, k0 = r - s_off[lo];
                 t.table[(size_t)s_slot[lo] * t.max_pages + s_first[lo] + k0] = id;
                 t.refs[id] = 1;  // read by this thread alone in this walk
                 if (k0 == 0) s_to[lo] = id;
@@ -390,7 +381,11 @@ hipError_t lk_pages_fork_launch(const LkPages& p, const LkTable& t, const uint32
 }
 hipError_t lk_pages_grow_launch(const LkPages& p, const LkTable& t, const uint32_t* slots, const uint32_t* add,
                                 uint32_t n, uint32_t* ok, uint32_t* copied, hipStream_t st) {
-    hipLaunchKernelGGL(pages_grow_kernel, dim3(1), dim3(kGrowThreads), 0, st, p, t, slots, add, n, ok, copied);
+    // a short list over few pages: fewer waves to wait for
+    if (n <= 256 && p.n_pages <= 8192)
+        hipLaunchKernelGGL((pages_grow_kernel<256>), dim3(1), dim3(256), 0, st, p, t, slots, add, n, ok, copied);
+    else
+        hipLaunchKernelGGL((pages_grow_kernel<1024>), dim3(1), dim3(1024), 0, st, p, t, slots, add, n, ok, copied);
     hipLaunchKernelGGL(pages_copy_kernel, dim3(n, p.n_layers, 2 * p.n_kv), dim3(256), 0, st, p, t, slots, add, copied);
     return hipGetLastError();
 }
