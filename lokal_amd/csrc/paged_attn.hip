@@ -234,6 +234,8 @@ struct Rows {
     }
     // k: f16 the lane's 8 dims 32 ks + 8 j of position c16, f32 its 4 dims 16 ks + 4 j.  Products that follow each other
     // belong to different sums.
+    // PARTS of q: 1 where k is the second part of K itself.
+    template <int PARTS = 2>
     __device__ __forceinline__ void scores(const u4 (&k)[NT], int ks, Scores& sc) const {
         if constexpr (F32) {
 #pragma unroll
@@ -245,7 +247,7 @@ struct Rows {
                         sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, k[t])[e], qf[rt][ks][e], sc[rt][t], 0, 0, 0);
         } else {
 #pragma unroll
-            for (int part = 0; part < 2; part++)
+            for (int part = 0; part < PARTS; part++)
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -354,11 +356,12 @@ struct Rows {
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) lr[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[rt], ones, lr[rt], 0, 0, 0);
     }
-    // vb: column tiles d0.. of their V, positions 4 j + i of the one tile, then of the other
-    template <int N>
+    // vb: column tiles d0.. of their V, positions 4 j + i of the one tile, then of the other.  PARTS of the weights: 1
+    // where vb is V's second part.
+    template <int PARTS = 2, int N>
     __device__ __forceinline__ void add16(const h8 (&ph)[RT], const h8 (&pl)[RT], const h8 (&vb)[N], int d0) {
 #pragma unroll
-        for (int part = 0; part < 2; part++)
+        for (int part = 0; part < PARTS; part++)
 #pragma unroll
             for (int d = 0; d < N; d++)
 #pragma unroll
@@ -404,6 +407,7 @@ struct Rows {
     }
     // Rows that see a value that is not finite, in a step that had something to hide: NaN in its dim.  Rare, so short: a
     // position at a time, after all steps.
+    template <bool OF32>  // the cache's type
     __device__ __forceinline__ void poison(const LkPagedAttn& a, const Share& h, uint32_t x) {
         uint64_t live = 0;
         bool masked = false;
@@ -425,7 +429,7 @@ struct Rows {
             for (int d = 0; d < ND; d++) {
                 const uint64_t e = at + dim_of<HD, F32, TR>(c16, d);
                 bool b;
-                if constexpr (F32) b = not_finite(((const float*)a.p.v)[e]);
+                if constexpr (OF32) b = not_finite(((const float*)a.p.v)[e]);
                 else b = (((const uint16_t*)a.p.v)[e] & 0x7C00) == 0x7C00;
                 bad |= (uint32_t)b << d;
             }
@@ -590,7 +594,7 @@ __global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow
         use(x, k, v, live, masked, scaled);
     }
     if (!SPARSE && __any(odd))
-        for (x = h.x0 + w * STEP; x < h.x1; x += W * STEP) r.poison(a, h, x);
+        for (x = h.x0 + w * STEP; x < h.x1; x += W * STEP) r.template poison<F32>(a, h, x);
     // ---- the waves join: m and sum per row, then O one wave after the other
 #pragma unroll
     for (int rt = 0; rt < RT; rt++)
@@ -745,17 +749,23 @@ __device__ __forceinline__ Plan plan_runs(const LkPagedAttn& a, uint32_t wg, uin
 template <int HD, bool F32, int NW>
 struct Wide {
     static constexpr int NT = F32 || HD == 128 ? 2 : 4, STEP = NT * 16, ROWS = NW * 32;
+    static constexpr int SIDE = STEP * HD * (F32 ? 4 : 2);  // bytes of a step's K or V
+    static constexpr int RING = F32 ? 1 : SIDE <= 8192 && NW == 4 ? 3 : 2;
 };
 template <int HD, bool F32, int NW>
 __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const LkPagedAttn a) {
     constexpr int RT = 2, NT = Wide<HD, F32, NW>::NT, STEP = Wide<HD, F32, NW>::STEP, ROWS = Wide<HD, F32, NW>::ROWS;
-    using Wave = Rows<HD, F32, RT, NT, false, !F32>;
-    constexpr int ND = Wave::ND, KS = Wave::KS, VW = Wave::VW, ES = Wave::ES;
+    using Wave = Rows<HD, false, RT, NT, false, true>;
+    constexpr int ND = Wave::ND, KS = Wave::KS, ES = F32 ? 4 : 2;
     constexpr int RB = HD * ES, PIECES = RB / 16, PER = 64 / PIECES;  // rows that one load instruction covers
     constexpr int SIDE = STEP * RB, OPS = SIDE / 1024 / NW;           // a step's K or V; a wave's loads of it
-    constexpr int RING = SIDE * NW <= 8192 * 4 && NW == 4 ? 3 : 2;
+    constexpr int RING = Wide<HD, F32, NW>::RING;
     static_assert(OPS >= 1 && SIDE % (1024 * NW) == 0 && 16 % PER == 0, "whole load instructions, each within a tile");
+    // f16: K, then V.  f32: one stage as it comes, and K and V in two f16 parts each.
+    constexpr int ROW = HD * 2, PART = STEP * ROW, V0 = F32 ? 2 * PART : SIDE;
     __shared__ __align__(1024) char ring[RING][2 * SIDE];
+    __shared__ __align__(1024) char s_parts[F32 ? 4 * PART : 16];
+    __shared__ float s_top[2][NW];
     __shared__ uint32_t s_odd;  // a V that is not finite was met
     typedef __attribute__((address_space(3))) uint32_t* lptr;
     typedef __attribute__((address_space(1))) uint32_t* gptr;
@@ -827,7 +837,7 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
             for (int k = 0; k < 2 * OPS; k++) {
                 const uint32_t q = w * OPS + k % OPS, row0 = q * PER, tile = (n * NT + row0 / 16) & 63;
                 const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, tile) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, tile);
-                const uint32_t mine = ((row0 & 15) + in_op) * RB + ((my_piece ^ ((row0 + in_op) & 7)) * 16);
+                const uint32_t mine = ((row0 & 15) + in_op) * RB + ((F32 ? my_piece : my_piece ^ ((row0 + in_op) & 7)) * 16);
                 const char* from = (const char*)(k < OPS ? a.p.k : a.p.v) + at;
                 __builtin_amdgcn_global_load_lds((gptr)(from + mine), (lptr)(to + (k < OPS ? 0 : SIDE) + q * 1024), 16, 0, 0);
             }
@@ -850,9 +860,10 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
         };
         __syncthreads();  // the last part's s_odd is read
         if (threadIdx.x == 0) s_odd = 0;  // set behind a barrier at the earliest
-        uint32_t tiles[RING - 1];  // of the steps under way: which tiles are no holes
+        constexpr int AHEAD = F32 ? 1 : RING - 1;
+        uint32_t tiles[AHEAD];  // of the steps under way: which tiles are no holes
 #pragma unroll
-        for (int n = 0; n < RING - 1; n++) {
+        for (int n = 0; n < AHEAD; n++) {
             tiles[n] = 0;
             if ((uint32_t)n < steps) {
                 tiles[n] = look(n);
@@ -861,93 +872,178 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
         }
         Wave r;
         const bool scaled = r.init(a, h, rbase);
-        // Where the lane reads a stage: K piece 4 ks + j of row c16; V f32: its dims of row 4 j + i, V f16: the part of
-        // column tile d that it hands the transposing read (of 16 lanes, four hold a row's 16 dims, and each gets one
-        // dim of the four rows).  A tile further is 16 rows on.
-        uint32_t k_at[KS], v_at[F32 ? 4 : ND][VW > 4 ? 2 : 1];
+        // Where the lane reads: K piece 4 ks + j of row c16; of V the part of column tile d that it hands the transposing
+        // read (of 16 lanes, four hold a row's 16 dims, and each gets one dim of the four rows).  A tile further is 16
+        // rows on.
+        uint32_t k_at[KS], v_at[ND];
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) k_at[ks] = r.c16 * RB + ((4 * ks + r.j) ^ (r.c16 & 7)) * 16;
-        if constexpr (F32) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t row = 4 * r.j + i;
-#pragma unroll
-                for (int d = 0; d < VW; d += 4) v_at[i][d / 4] = SIDE + row * RB + ((4 * d + r.c16) ^ (row & 7)) * 16;
-            }
-        } else {
+        for (int ks = 0; ks < KS; ks++) k_at[ks] = r.c16 * ROW + ((4 * ks + r.j) ^ (r.c16 & 7)) * 16;
+        {
             const uint32_t row = 4 * r.j + r.c16 / 4;
 #pragma unroll
-            for (int d = 0; d < ND; d++) v_at[d][0] = SIDE + row * RB + ((2 * d + r.c16 % 4 / 2) ^ (row & 7)) * 16 + (r.c16 & 1) * 8;
+            for (int d = 0; d < ND; d++) v_at[d] = V0 + row * ROW + ((2 * d + r.c16 % 4 / 2) ^ (row & 7)) * 16 + (r.c16 & 1) * 8;
         }
+        int v_up = 100;  // f32: O is in units of 2^-v_up
         uint32_t slot = 0;  // n % RING
         for (uint32_t n = 0; n < steps; n++) {
             // step n has landed for every wave, and every wave is done with the stage that is filled next
-            if (RING > 2 && n + RING - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * 2 * OPS) : "memory");
+            if (!F32 && RING > 2 && n + RING - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * 2 * OPS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             const uint32_t tl = tiles[0];
 #pragma unroll
-            for (int k = 0; k + 1 < RING - 1; k++) tiles[k] = tiles[k + 1];
-            if (n + RING - 1 < steps) {
-                turn_page(n + RING - 1);
-                tiles[RING - 2] = look(n + RING - 1);
-                issue(n + RING - 1, ring[slot ? slot - 1 : RING - 1]);
-            }
-            char* stage = ring[slot];
-            slot = slot + 1 < RING ? slot + 1 : 0;
+            for (int k = 0; k + 1 < AHEAD; k++) tiles[k] = tiles[k + 1];
             const uint32_t x = h.x0 + n * STEP;
             const bool masked = tl != (1u << NT) - 1 || x + STEP > h.sq.ctx;  // uniform: something to hide
-            uint64_t live = 0;
-            if (masked) {
-                // V of positions that no row sees becomes zero, and what is not finite too
-                live = live_of(x, tl);
+            const uint64_t live = masked ? live_of(x, tl) : 0;
+            char* stage;
+            int k_up = 0;  // f32: K was taken times 2^k_up
+            if constexpr (F32) {
+                // K and V into f16 parts, each step's largest value brought to 2^13..2^14: 22 bits of those near it, and
+                // 2^-39 of it for the others.  V's power only falls, O following it.
+                stage = s_parts;
+                constexpr uint32_t UNITS = STEP * HD / 8, EACH = (UNITS + NW * 64 - 1) / (NW * 64);
+                f4 u[2][EACH][2];
+                float top[2] = {0.f, 0.f};
                 uint32_t any = 0;
-                for (uint32_t p = threadIdx.x; p < SIDE / 16; p += NW * 64) {
-                    u4* at = (u4*)(stage + SIDE + p * 16);
-                    u4 y = *at;
-                    const bool see = live >> (p / PIECES) & 1;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] = Wave::clean_word(see ? y[e] : 0, any);
-                    *at = y;
+                for (int side = 0; side < 2; side++)
+#pragma unroll
+                    for (uint32_t e = 0; e < EACH; e++) {
+                        const uint32_t at = threadIdx.x + e * NW * 64, row = at / (HD / 8);
+                        const f4* from = (const f4*)(ring[0] + side * SIDE + at * 32);
+                        const bool see = !side || !masked || live >> row & 1;
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            f4 y = from[k];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const bool bad = not_finite(y[i]);
+                                if (side && masked) {
+                                    any |= see && bad;
+                                    y[i] = see && !bad ? y[i] : 0.f;
+                                }
+                                top[side] = fmaxf(top[side], bad ? 0.f : fabsf(y[i]));
+                            }
+                            u[side][e][k] = y;
+                        }
+                    }
+#pragma unroll
+                for (int side = 0; side < 2; side++) {
+                    const float t = lk_wave_max(top[side]);
+                    if (lane == 0) s_top[side][w] = t;
                 }
                 if (any) s_odd = 1;
+                __syncthreads();  // the stage is read: the next one may come
+                if (n + 1 < steps) {
+                    turn_page(n + 1);
+                    tiles[0] = look(n + 1);
+                    issue(n + 1, ring[0]);
+                }
+                int up[2];
+#pragma unroll
+                for (int side = 0; side < 2; side++) {
+                    float t = s_top[side][0];
+#pragma unroll
+                    for (int k = 1; k < NW; k++) t = fmaxf(t, s_top[side][k]);
+                    const int e = 13 + 127 - (int)(__float_as_uint(t) >> 23);
+                    up[side] = __builtin_amdgcn_readfirstlane(t > 0.f ? (e < 100 ? e : 100) : 100);
+                }
+                k_up = up[0];
+                if (up[1] < v_up) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                        for (int d = 0; d < ND; d++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) r.o[rt][d][i] = ldexpf(r.o[rt][d][i], up[1] - v_up);
+                    v_up = up[1];
+                }
+                up[1] = v_up;
+#pragma unroll
+                for (int side = 0; side < 2; side++)
+#pragma unroll
+                    for (uint32_t e = 0; e < EACH; e++) {
+                        const uint32_t at = threadIdx.x + e * NW * 64, row = at / (HD / 8), piece = (at % (HD / 8)) ^ (row & 7);
+                        h8 hi, lo;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float y = ldexpf(u[side][e][i / 4][i % 4], up[side]);
+                            hi[i] = (_Float16)y;
+                            lo[i] = (_Float16)(y - (float)hi[i]);
+                        }
+                        char* to = s_parts + side * 2 * PART + row * ROW + piece * 16;
+                        *(h8*)to = hi;
+                        *(h8*)(to + PART) = lo;
+                    }
                 __syncthreads();
+            } else {
+                if (n + RING - 1 < steps) {
+                    turn_page(n + RING - 1);
+                    tiles[AHEAD - 1] = look(n + RING - 1);
+                    issue(n + RING - 1, ring[slot ? slot - 1 : RING - 1]);
+                }
+                stage = ring[slot];
+                slot = slot + 1 < RING ? slot + 1 : 0;
+                if (masked) {
+                    // V of positions that no row sees becomes zero, and what is not finite too
+                    uint32_t any = 0;
+                    for (uint32_t p = threadIdx.x; p < SIDE / 16; p += NW * 64) {
+                        u4* at = (u4*)(stage + SIDE + p * 16);
+                        u4 y = *at;
+                        const bool see = live >> (p / PIECES) & 1;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[e] = Wave::clean_word(see ? y[e] : 0, any);
+                        *at = y;
+                    }
+                    if (any) s_odd = 1;
+                    __syncthreads();
+                }
             }
             if (!busy) continue;
             f4 sc[RT][NT];
-            r.start(sc);
+            if constexpr (F32) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++) sc[rt][t] = f4{0.f, 0.f, 0.f, 0.f};
+            } else {
+                r.start(sc);
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 u4 kr[NT];
 #pragma unroll
-                for (int t = 0; t < NT; t++) kr[t] = *(const u4*)(stage + k_at[ks] + t * 16 * RB);
+                for (int t = 0; t < NT; t++) kr[t] = *(const u4*)(stage + k_at[ks] + t * 16 * ROW);
                 r.scores(kr, ks, sc);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++) kr[t] = *(const u4*)(stage + PART + k_at[ks] + t * 16 * ROW);
+                    r.template scores<1>(kr, ks, sc);
+                }
                 if (HD == 128 && ks % 2) __builtin_amdgcn_sched_barrier(0);  // K operands of two at a time: registers
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    const int by = -(r.up[rt] + k_up);  // scores of 2^126 and more are all alike
+                    const float f = ldexpf(1.f, by < 126 ? by : 126), z = r.m[rt] == -INFINITY ? 0.f : -r.m[rt];
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sc[rt][t][i] = fmaf(sc[rt][t][i], f, z);
+                }
             }
             if (masked) {
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt), sc);
             }
-            r.move(sc, scaled);
-            if constexpr (F32) {
+            r.move(sc, !F32 && scaled);
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+            for (int g = 0; g < NT / 2; g++) {
+                h8 ph[RT], pl[RT];
+                r.weights(sc, g, ph, pl);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t y[VW];
-#pragma unroll
-                        for (int d = 0; d < VW; d += 4) {
-                            const u4 z = *(const u4*)(stage + v_at[i][d / 4] + t * 16 * RB);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) y[d + e] = z[e];
-                        }
-                        r.add32(sc, t, i, y);
-                        if (HD == 128 && i % 2) __builtin_amdgcn_sched_barrier(0);
-                    }
-            } else {
-#pragma unroll
-                for (int g = 0; g < NT / 2; g++) {
-                    h8 ph[RT], pl[RT];
-                    r.weights(sc, g, ph, pl);
+                for (int part = 0; part < (F32 ? 2 : 1); part++)
 #pragma unroll
                     for (int d0 = 0; d0 < ND; d0 += 4) {
                         h8 vb[4];
@@ -956,18 +1052,18 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
                             u2 y[2];
 #pragma unroll
                             for (int t = 0; t < 2; t++)
-                                y[t] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((sptr)(stage + v_at[d0 + d][0] + (2 * g + t) * 16 * RB)));
+                                y[t] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((sptr)(stage + part * PART + v_at[d0 + d] + (2 * g + t) * 16 * ROW)));
                             vb[d] = __builtin_bit_cast(h8, u4{y[0][0], y[0][1], y[1][0], y[1][1]});
                         }
-                        r.add16(ph, pl, vb, d0);
+                        if (part == 0) r.add16(ph, pl, vb, d0);
+                        else r.template add16<1>(ph, pl, vb, d0);
                         if (HD == 128) __builtin_amdgcn_sched_barrier(0);
                     }
-                }
             }
         }
         __syncthreads();  // s_odd, and the stages, are settled
         if (s_odd && busy)
-            for (uint32_t n = 0; n < steps; n++) r.poison(a, h, h.x0 + n * STEP);
+            for (uint32_t n = 0; n < steps; n++) r.template poison<F32>(a, h, h.x0 + n * STEP);
         if (!busy) continue;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
@@ -975,7 +1071,7 @@ __global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const 
             for (int i = 0; i < 4; i++) {
                 float y[ND];
 #pragma unroll
-                for (int d = 0; d < ND; d++) y[d] = r.o[rt][d][i];
+                for (int d = 0; d < ND; d++) y[d] = F32 ? ldexpf(r.o[rt][d][i], -v_up) : r.o[rt][d][i];
                 const float top = r.max_of(rt, i), sum = r.sum_of(rt, i);
                 r.put(a, h, w * 32 + rt * 16 + 4 * r.j + i, top, sum, y);
             }
