@@ -652,10 +652,8 @@ __device__ __forceinline__ uint32_t item_steps(const Seq& q, uint32_t step) { re
 __device__ __forceinline__ uint32_t row_groups(const LkPagedAttn& a, const Seq& q, uint32_t rows) {
     return q.live ? (q.rows * a.G + rows - 1) / rows : 0;
 }
-#ifndef LK_LEAST
-#define LK_LEAST 2
-#endif
-constexpr uint32_t kLeast = LK_LEAST;  // steps of a run at least
+constexpr uint32_t kLeast = 2;  // steps of a run at least
+constexpr uint32_t kOcc = 2;    // waves of the wide kernel on a SIMD: 256 registers each
 
 // All workgroups count all sequences; `start`: where this one's run begins.  Sequences are read twice (total, then
 // the place) unless one round of the threads holds them.  Workgroup 0 leaves the sequences' places for the fold.
@@ -743,9 +741,6 @@ __device__ __forceinline__ Plan plan_runs(const LkPagedAttn& a, uint32_t wg, uin
 // ahead; one barrier a step.  A place there holds rows of RB bytes, whose 16-byte pieces lie at their number ^ (row &
 // 7), so that eight lanes that read one piece of eight rows meet eight different bank groups.  Loads write LDS in lane
 // order, so the lane that lands in a place fetches the piece that belongs there.
-#ifndef LK_WIDE_OCC
-#define LK_WIDE_OCC 2
-#endif
 template <int HD, bool F32, int NW>
 struct Wide {
     static constexpr int NT = F32 || HD == 128 ? 2 : 4, STEP = NT * 16, ROWS = NW * 32;
@@ -753,7 +748,7 @@ struct Wide {
     static constexpr int RING = F32 ? 1 : SIDE <= 8192 && NW == 4 ? 3 : 2;
 };
 template <int HD, bool F32, int NW>
-__global__ __launch_bounds__(NW * 64, LK_WIDE_OCC) void paged_wide_kernel(const LkPagedAttn a) {
+__global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPagedAttn a) {
     constexpr int RT = 2, NT = Wide<HD, F32, NW>::NT, STEP = Wide<HD, F32, NW>::STEP, ROWS = Wide<HD, F32, NW>::ROWS;
     using Wave = Rows<HD, false, RT, NT, false, true>;
     constexpr int ND = Wave::ND, KS = Wave::KS, ES = F32 ? 4 : 2;
@@ -1148,9 +1143,13 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
     p.rows_pad = p.n_rg * per;
     const uint64_t base = (uint64_t)n * n_kv * p.n_rg;
     const uint32_t step = f32 || hd == 128 ? 32 : 64;
-    const uint64_t steps = (positions + step - 1) / step, fill = (uint64_t)kCus * LK_WIDE_OCC * 4 / p.waves;
+    const uint64_t steps = (positions + step - 1) / step, fill = (uint64_t)kCus * kOcc * 4 / p.waves;
     p.steps = base * steps;
-    if (!p.narrow && p.steps > (f32 ? 4 : 16) * fill) {
+    // Runs begin 7 us later than chunks (they count the work first) and pay from about 480 positions a workgroup on, 240
+    // of an f32 cache.  us, chunks / runs: 4 x 32 tokens, 32 / 4 heads of 64, up to 4096 positions (256 a workgroup) 25 /
+    // 30, 8192 (512) 44 / 35; 24 x 12, 32 / 8 of 128, 2048 (390) 51 / 59, 8 x 16, 8192 (512) 80 / 74; f32, 3 x 23, 32 / 8
+    // of 128, 5000 (236) 59 / 64, 4 x 16, 8192 (256) 169 / 100.
+    if (!p.narrow && p.steps * step > (f32 ? 240 : 480) * fill) {
         p.blocks = fill;
         p.part_rows = fill * 2 * per;
         p.place_bytes = (((uint64_t)n + 1) * 8 + 255) / 256 * 256;
