@@ -424,8 +424,9 @@ int lkhip_pages_compact(const lkhip_kv_pages* pages, const lkhip_page_table* tab
  * the drafted tokens j < n_draft[i] whose bit is set: bit j % 32 of
  * mask[i][t][j / 32], [n][max_draft][ceil(max_draft / 32)] words; mask NULL: j
  * <= t.  Softmax of q.k / sqrt(head_dim) in f32; a row that sees nothing gives
- * zeros; rows at and behind n_draft[i] are left as they were.  n_draft NULL: all have max_draft (<= 1024).
- * n_heads: a multiple of the kv heads.  Positions that a row does not see do
+ * zeros; rows at and behind n_draft[i] are left as they were.  n_draft NULL: all
+ * have max_draft.  max_draft <= 1024; n_heads a multiple of the kv heads, at most
+ * 65536 / max_draft for each of them.  Positions that a row does not see do
  * not reach it, whatever they hold; one that it sees with a K or V that is not
  * finite makes it not finite.  Needs lkhip_tree_attn_workspace bytes (16-byte
  * aligned, any content), in use until the call's work is done: two calls that

@@ -188,6 +188,9 @@ static int attn_shape(const LkPages& p, size_t n, size_t tokens, size_t n_heads,
         return fail(LKHIP_E_UNSUPPORTED, "%s: %zu query heads over %u kv heads — a multiple of them, at most 4096", who,
                     n_heads, p.n_kv);
     if (tokens > 1024) return fail(LKHIP_E_UNSUPPORTED, "%s: %zu drafted tokens — at most 1024", who, tokens);
+    if (tokens * (n_heads / p.n_kv) > 0x10000)
+        return fail(LKHIP_E_UNSUPPORTED, "%s: %zu drafted tokens x %zu query heads of a kv head — at most 65536 rows", who,
+                    tokens, n_heads / p.n_kv);
     return LKHIP_OK;
 }
 static int plan_of(const LkPages& p, const LkTable& t, size_t n, size_t tokens, size_t n_heads, size_t take,
@@ -199,7 +202,8 @@ static int plan_of(const LkPages& p, const LkTable& t, size_t n, size_t tokens, 
     keys = take ? (size_t)n * p.n_kv * t.max_pages * 8 : 0;
     keys = (keys + 255) / 256 * 256;
     bytes = keys + plan.part_bytes;
-    if (plan.blocks > 0x7FFFFFFF || (uint64_t)n * p.n_kv * (plan.n_chunks + 1) > 0x7FFFFFFF || plan.steps > 0xFFFFFFFF)
+    // grids of 256 threads a block, below 2^32 threads; steps are counted in 32 bits
+    if (plan.blocks > 0xFFFFFF || (uint64_t)n * p.n_kv * (plan.n_chunks + 1) > 0xFFFFFF || plan.steps > 0xFFFFFFFF)
         return fail(LKHIP_E_INVALID, "%s: %zu sequences x %zu tokens x %zu heads over %llu positions are too many for one call",
                     who, n, tokens, n_heads, (unsigned long long)cap);
     return LKHIP_OK;

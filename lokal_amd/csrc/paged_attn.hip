@@ -153,18 +153,15 @@ struct Rows {
     h8 qh[F32 ? 1 : RT][F32 ? 1 : KS], ql[F32 ? 1 : RT][F32 ? 1 : KS];
     f4 qf[F32 ? RT : 1][F32 ? ND : 1];
     float m[RT];     // log2: what row c16's weights are relative to; -inf before its first score
-    float l[F32 ? RT : 1];  // lane's part of row c16's sum
-    f4 lr[F32 ? 1 : RT];    // sums of rows 4 j + i, by a product with ones: the matrix cores have time, the adders not
+    float l[RT];     // lane's part of row c16's sum: on the adders, which round; the matrix cores' long sums drift
     uint32_t tok[RT];
     f4 o[RT][ND];
     int up[RT];      // q was taken times 2^up: 0 for rows whose largest value needs no scaling
     uint32_t j, c16;
     using Scores = f4[RT][NT];
 
-    // Whether some row's up is not 0.
-    __device__ __forceinline__ bool init(const LkPagedAttn& a, const Share& h, uint32_t rbase) {
+    __device__ __forceinline__ void init(const LkPagedAttn& a, const Share& h, uint32_t rbase) {
         j = (threadIdx.x & 63) >> 4, c16 = threadIdx.x & 15;
-        bool scaled = false;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const uint32_t row = rbase + rt * 16 + c16;
@@ -173,8 +170,8 @@ struct Rows {
             const uint32_t g = live ? row - tok[rt] * a.G : 0;
             const float* q = a.q + (((size_t)h.s * a.tokens + tok[rt]) * a.n_heads + h.kvh * a.G + g) * HD;
             m[rt] = -INFINITY;
-            if constexpr (F32) l[rt] = 0.f, up[rt] = 0;
-            else lr[rt] = f4{0.f, 0.f, 0.f, 0.f};
+            l[rt] = 0.f;
+            up[rt] = 0;
 #pragma unroll
             for (int d = 0; d < ND; d++) o[rt][d] = f4{0.f, 0.f, 0.f, 0.f};
             if constexpr (F32) {
@@ -208,7 +205,6 @@ struct Rows {
                         for (int e = 0; e < 8; e++) x[ks][e] = ldexpf(x[ks][e], by);
                 }
                 up[rt] = by;
-                scaled |= __any(by != 0);
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -219,18 +215,13 @@ struct Rows {
                     }
             }
         }
-        return scaled;
     }
 
-    // Scores relative to m: the products start at -m.
-    __device__ __forceinline__ void start(Scores& sc) const {
+    static __device__ __forceinline__ void start(Scores& sc) {
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            float z = m[rt] == -INFINITY ? 0.f : -m[rt];
-            if constexpr (!F32) z = ldexpf(z, up[rt]);
+        for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-            for (int t = 0; t < NT; t++) sc[rt][t] = f4{z, z, z, z};
-        }
+            for (int t = 0; t < NT; t++) sc[rt][t] = f4{0.f, 0.f, 0.f, 0.f};
     }
     // k: f16 the lane's 8 dims 32 ks + 8 j of position c16, f32 its 4 dims 16 ks + 4 j.  Products that follow each other
     // belong to different sums.
@@ -287,18 +278,24 @@ struct Rows {
             for (int i = 0; i < 4; i++) sc[rt][t][i] = b[t / 2] >> (16 * (t & 1) + i) & 1 ? sc[rt][t][i] : -INFINITY;
     }
 
+    // Products of K times 2^k_up become scores relative to m.
+    __device__ __forceinline__ void relate(Scores& sc, int k_up) const {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const int by = -(up[rt] + k_up);  // scores of 2^126 and more are all alike
+            const float f = ldexpf(1.f, by < 126 ? by : 126), z = m[rt] == -INFINITY ? 0.f : -m[rt];
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[rt][t][i] = fmaf(sc[rt][t][i], f, z);
+        }
+    }
     // Before scores become weights: m moves up where one passes it by kLag.
-    __device__ __forceinline__ void move(Scores& sc, bool scaled) {
+    __device__ __forceinline__ void move(Scores& sc) {
         float top[RT];
         bool far = false;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            if (!F32 && scaled) {
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sc[rt][t][i] = ldexpf(sc[rt][t][i], -up[rt]);
-            }
             top[rt] = -INFINITY;
 #pragma unroll
             for (int t = 0; t < NT; t++)
@@ -318,11 +315,10 @@ struct Rows {
             m[rt] = first ? x : m[rt] + by;
 #pragma unroll
             for (int t = 0; t < NT; t++) sc[rt][t] -= by;
-            if constexpr (F32) l[rt] *= f;
+            l[rt] *= f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float fi = __shfl(f, (int)(4 * j + i), 64);  // O's rows are 4 j + i
-                if constexpr (!F32) lr[rt][i] *= fi;
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[rt][d][i] *= fi;
             }
@@ -331,9 +327,6 @@ struct Rows {
 
     // f16: the weights of tiles 2 g and 2 g + 1 in two parts, and their sums.
     __device__ __forceinline__ void weights(const Scores& sc, int g, h8 (&ph)[RT], h8 (&pl)[RT]) {
-        h8 ones;
-#pragma unroll
-        for (int e = 0; e < 8; e++) ones[e] = (_Float16)1.f;
         float minus = -1.f;  // a register: p - hi is then one mixed product, hi not widened first
         asm("" : "+s"(minus));
 #pragma unroll
@@ -343,6 +336,7 @@ struct Rows {
             for (int e = 0; e < 4; e++) {  // truncated to f16; what that leaves fits f16's 11 bits but for two
                 const float p0 = __builtin_amdgcn_exp2f(sc[rt][2 * g + e / 2][2 * (e & 1)]),
                             p1 = __builtin_amdgcn_exp2f(sc[rt][2 * g + e / 2][2 * (e & 1) + 1]);
+                l[rt] += p0 + p1;
                 const p2 u = __builtin_amdgcn_cvt_pkrtz(p0, p1);
                 hi[e] = __builtin_bit_cast(uint32_t, u);
                 lo[e] = __builtin_bit_cast(
@@ -351,10 +345,6 @@ struct Rows {
             ph[rt] = __builtin_bit_cast(h8, u4{hi[0], hi[1], hi[2], hi[3]});
             pl[rt] = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
         }
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) lr[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[rt], ones, lr[rt], 0, 0, 0);
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) lr[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[rt], ones, lr[rt], 0, 0, 0);
     }
     // vb: column tiles d0.. of their V, positions 4 j + i of the one tile, then of the other.  PARTS of the weights: 1
     // where vb is V's second part.
@@ -449,14 +439,10 @@ struct Rows {
 
     // Sum of row 4 j + i of tile rt, on its lanes.
     __device__ __forceinline__ float sum_of(int rt, int i) const {
-        if constexpr (F32) {
-            float x = l[rt];
-            x += __shfl_xor(x, 16, 64);
-            x += __shfl_xor(x, 32, 64);
-            return __shfl(x, (int)(4 * j + i), 64);
-        } else {
-            return lr[rt][i];
-        }
+        float x = l[rt];
+        x += __shfl_xor(x, 16, 64);
+        x += __shfl_xor(x, 32, 64);
+        return __shfl(x, (int)(4 * j + i), 64);
     }
     __device__ __forceinline__ float max_of(int rt, int i) const { return __shfl(m[rt], (int)(4 * j + i), 64); }
     // Row lr of the workgroup: the output where the sequence has one chunk, else the chunk's (m, sum, O).
@@ -540,7 +526,7 @@ __global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow
             }
     };
     uint32_t odd = 0;
-    auto use = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t live, bool masked, bool scaled) LK_INLINE {
+    auto use = [&](uint32_t x, u4 (&k)[NT][KS], uint32_t (&v)[NT][4][VW], uint64_t live, bool masked) LK_INLINE {
         f4 sc[RT][NT];
         r.start(sc);
 #pragma unroll
@@ -550,6 +536,7 @@ __global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow
             for (int t = 0; t < NT; t++) kk[t] = k[t][ks];
             r.scores(kk, ks, sc);
         }
+        r.relate(sc, 0);
         if (__builtin_amdgcn_readfirstlane(masked)) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt), sc);
@@ -558,7 +545,7 @@ __global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow
 #pragma unroll
                 for (int i = 0; i < 4; i++) odd |= r.clean(t, i, live, v[t][i]);
         }
-        r.move(sc, scaled);
+        r.move(sc);
         if constexpr (F32) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
@@ -583,7 +570,7 @@ __global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow
             }
         }
     };
-    const bool scaled = r.init(a, h, h.row0);
+    r.init(a, h, h.row0);
     uint32_t x = h.x0 + w * STEP;
     for (; x < h.x1; x += W * STEP) {
         u4 k[NT][KS];
@@ -591,7 +578,7 @@ __global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow
         uint64_t live;
         bool masked;
         fetch(x, k, v, live, masked);
-        use(x, k, v, live, masked, scaled);
+        use(x, k, v, live, masked);
     }
     if (!SPARSE && __any(odd))
         for (x = h.x0 + w * STEP; x < h.x1; x += W * STEP) r.template poison<F32>(a, h, x);
@@ -785,6 +772,7 @@ __global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPaged
         if (chunks) {
             steps = (h.x1 - h.x0 + STEP - 1) / STEP;
         } else {
+            if (seq >= a.n) return;  // uniform; not reached unless the lengths change under the call
             h.s = seq;
             h.sq = seq_of<false>(a, seq);
             const uint32_t groups = row_groups(a, h.sq, ROWS), of_item = groups ? item_steps(h.sq, STEP) : 0;
@@ -866,7 +854,7 @@ __global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPaged
             }
         }
         Wave r;
-        const bool scaled = r.init(a, h, rbase);
+        r.init(a, h, rbase);
         // Where the lane reads: K piece 4 ks + j of row c16; of V the part of column tile d that it hands the transposing
         // read (of 16 lanes, four hold a row's 16 dims, and each gets one dim of the four rows).  A tile further is 16
         // rows on.
@@ -996,14 +984,7 @@ __global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPaged
             }
             if (!busy) continue;
             f4 sc[RT][NT];
-            if constexpr (F32) {
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int t = 0; t < NT; t++) sc[rt][t] = f4{0.f, 0.f, 0.f, 0.f};
-            } else {
-                r.start(sc);
-            }
+            r.start(sc);
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 u4 kr[NT];
@@ -1017,22 +998,12 @@ __global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPaged
                 }
                 if (HD == 128 && ks % 2) __builtin_amdgcn_sched_barrier(0);  // K operands of two at a time: registers
             }
-            if constexpr (F32) {
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    const int by = -(r.up[rt] + k_up);  // scores of 2^126 and more are all alike
-                    const float f = ldexpf(1.f, by < 126 ? by : 126), z = r.m[rt] == -INFINITY ? 0.f : -r.m[rt];
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) sc[rt][t][i] = fmaf(sc[rt][t][i], f, z);
-                }
-            }
+            r.relate(sc, k_up);
             if (masked) {
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) r.hide(rt, r.sees(a, h, x, live, rt), sc);
             }
-            r.move(sc, !F32 && scaled);
+            r.move(sc);
 #pragma unroll
             for (int g = 0; g < NT / 2; g++) {
                 h8 ph[RT], pl[RT];

@@ -264,13 +264,13 @@ __global__ __launch_bounds__(256) void pages_compact_kernel(LkPages p, LkTable t
                                                             uint32_t ld_path, const uint32_t* n_path, uint32_t n) {
     __shared__ uint64_t s_from[64], s_to[64];  // elements within a layer's kv head; ~0: not moved
     __shared__ uint32_t s_rows;
-    const uint32_t i = blockIdx.x, s = slots[i];
+    const uint32_t i = blockIdx.y, s = slots[i];
     const uint64_t c0 = from[i];
     uint32_t count = n_path[i];
     count = count < ld_path ? count : ld_path;
     if (s >= t.n_seq || in_list(slots, i, s, n)) return;  // uniform
     const uint32_t es = p.f32 ? 4 : 2, cols = p.hd * es / 16;
-    const uint32_t u = blockIdx.y * 256 + threadIdx.x;
+    const uint32_t u = blockIdx.x * 256 + threadIdx.x;
     const uint32_t col = u % cols, hv = u / cols % (2 * p.n_kv), layer = u / cols / (2 * p.n_kv);
     char* const pool = (char*)(hv & 1 ? p.v : p.k) + (layer * p.layer_stride + (hv >> 1) * p.head_stride) * es + col * 16;
     const uint32_t* row = t.table + (size_t)s * t.max_pages;
@@ -408,7 +408,7 @@ hipError_t lk_pages_compact_launch(const LkPages& p, const LkTable& t, const uin
                                    const uint32_t* path, uint32_t ld_path, const uint32_t* n_path, uint32_t n,
                                    hipStream_t st) {
     const uint32_t units = p.n_layers * 2 * p.n_kv * (p.hd * (p.f32 ? 4 : 2) / 16);
-    hipLaunchKernelGGL(pages_compact_kernel, dim3(n, (units + 255) / 256), dim3(256), 0, st, p, t, slots, from, path,
+    hipLaunchKernelGGL(pages_compact_kernel, dim3((units + 255) / 256, n), dim3(256), 0, st, p, t, slots, from, path,
                        ld_path, n_path, n);
     return hipGetLastError();
 }

@@ -82,25 +82,27 @@ def test_long_context_in_many_chunks(t):
     close(got, R.tree_rows(c, 0, q, ctx, [2, 2], None, 7, np.zeros(q.shape)), R.attn_tol(64, 9000, q, c.k), c.v)
 
 
+@pytest.mark.parametrize("t,heads", [("f16", 4), ("f16", 32), ("f32", 4), ("f32", 32)])
 @pytest.mark.parametrize("scale", [1e-30, 1e-6, 300.0, 1e20])
-def test_queries_of_any_size(scale):
+def test_queries_of_any_size(scale, t, heads):
     """Tiny queries see everything alike, huge ones one position; neither leaves what two f16 parts hold."""
     rng = np.random.default_rng(5)
-    c = R.Cache(rng, [100], kv=2, hd=64).up()
-    q = (rng.standard_normal((1, 3, 4 * 64)) * scale).astype(np.float32)
-    got = run_tree(c, 0, q, [97], [3], None, 4)
-    want = R.tree_rows(c, 0, q, [97], [3], None, 4, np.zeros(q.shape))
+    c = R.Cache(rng, [100], kv=2, hd=64, f32=t == "f32").up()
+    q = (rng.standard_normal((1, 3, heads * 64)) * scale).astype(np.float32)
+    got = run_tree(c, 0, q, [97], [3], None, heads)
+    want = R.tree_rows(c, 0, q, [97], [3], None, heads, np.zeros(q.shape))
     if scale <= 300:
         close(got, want, R.attn_tol(64, 100, q, c.k), c.v)
     else:  # scores of 1e20: the best position alone; no other comes within an f32 step of it here
         close(got, want, 2.0 ** -20, c.v)
 
 
-@pytest.mark.parametrize("t,hd", [("f16", 64), ("f16", 128), ("f32", 64)])
-def test_what_a_row_does_not_see_does_not_reach_it(t, hd):
+@pytest.mark.parametrize("heads", [6, 16, 32])
+@pytest.mark.parametrize("t,hd", [("f16", 64), ("f16", 128), ("f32", 64), ("f32", 128)])
+def test_what_a_row_does_not_see_does_not_reach_it(t, hd, heads):
     """Draft tokens with NaN and infinite K / V, seen by some rows alone; masks that leave rows empty."""
     rng = np.random.default_rng(6)
-    T, heads, kv = 9, 6, 2
+    T, kv = 9, 2
     for ctx in (0, 5, 60, 130):
         c = R.Cache(rng, [ctx + T], kv=kv, hd=hd, f32=t == "f32")
         bad = {2: np.nan, 4: np.inf, 7: -np.inf}
@@ -126,10 +128,11 @@ def test_what_a_row_does_not_see_does_not_reach_it(t, hd):
             assert (got[0, 0] == 0).all()
 
 
+@pytest.mark.parametrize("heads", [2, 10, 25])
 @pytest.mark.parametrize("t,hd", [("f16", 64), ("f16", 128), ("f32", 64), ("f32", 128)])
-def test_values_that_are_not_finite_reach_only_rows_that_see_them(t, hd):
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(t, hd, heads):
     rng = np.random.default_rng(16)
-    T, heads, kv, ctx = 5, 2, 1, 20
+    T, kv, ctx = 5, 1, 20
     c = R.Cache(rng, [ctx + T], kv=kv, hd=hd, f32=t == "f32")
     c.v[0, c.table[0, (ctx + 1) // c.page], 0, (ctx + 1) % c.page, 5] = np.nan
     c.up()
@@ -243,6 +246,119 @@ def test_pages_past_32_bit_offsets(kv_type):
     want = np.zeros((3, kv, 2, hd), t)
     R.bounds_of(c, 0, 0, 0, n, want)
     assert np.array_equal(bounds.numpy(), want)
+
+
+@pytest.mark.parametrize("heads", [2, 24])
+def test_f32_values_of_any_size(heads):
+    """Keys and values whose size changes from page to page by many powers of ten, either way, among them nothing but
+    zeros; and all of one size, far from 1."""
+    rng = np.random.default_rng(25)
+    T, hd, sizes = 3, 64, [1e-12, 1.0, 0.0, 1e9, 1e-3, 1e30, 1e-30]
+    for order in (sizes, sizes[::-1]):
+        c = R.Cache(rng, [32 * len(order) + T], kv=1, hd=hd, page=32, f32=True)
+        for x, size in enumerate(order):
+            c.v[0, c.table[0, x]] *= np.float32(size)
+        for x in range(0, len(order), 2):
+            c.k[0, c.table[0, x]] *= np.float32(1e-20)
+        c.up()
+        q = rng.standard_normal((1, T, heads * hd)).astype(np.float32)
+        ctx = 32 * len(order)
+        got = run_tree(c, 0, q, [ctx], [T], None, heads)
+        want = R.tree_rows(c, 0, q, [ctx], [T], None, heads, np.zeros(q.shape))
+        close(got, want, R.attn_tol(hd, ctx + T, q, c.k), c.v)
+    # one size at a time
+    for size in (1e-30, 1e-9, 1e25):
+        c = R.Cache(rng, [40 + T], kv=1, hd=hd, f32=True)
+        c.v *= np.float32(size)
+        c.k *= np.float32(1 / size if size < 1 else 1)
+        c.up()
+        q = (rng.standard_normal((1, T, heads * hd)) * min(size, 1)).astype(np.float32)
+        got = run_tree(c, 0, q, [40], [T], None, heads)
+        want = R.tree_rows(c, 0, q, [40], [T], None, heads, np.zeros(q.shape))
+        close(got, want, R.attn_tol(hd, 40 + T, q * (1 / min(size, 1)), c.k * min(size, 1)), c.v)
+
+
+def ragged(rng, n, most, T):
+    """Lengths of a batch: short ones, a few long, some without a draft."""
+    ctx = [int(x) for x in rng.integers(0, 60, n)]
+    for i in rng.integers(0, n, 5):
+        ctx[i] = int(rng.integers(most // 2, most))
+    nd = [int(x) for x in rng.integers(0, T + 1, n)]
+    return ctx, nd
+
+
+@pytest.mark.parametrize("t,hd,heads,kv,T,n", [("f16", 64, 8, 1, 16, 300), ("f16", 64, 16, 2, 20, 7), ("f16", 128, 6, 1, 8, 160),
+                                               ("f16", 128, 16, 2, 30, 5), ("f32", 64, 16, 2, 12, 9), ("f32", 128, 5, 1, 9, 6)])
+def test_long_tables_over_runs_of_steps(t, hd, heads, kv, T, n):
+    """Tables long enough that the work is counted on the device and dealt out in equal runs: many short sequences, a few
+    long ones, some with nothing to do, one without a slot, more of them than a workgroup has threads."""
+    rng = np.random.default_rng(n + hd)
+    ctx, nd = ragged(rng, n, 1500 if n > 100 else 4000, T)
+    ctx[0] = 1500
+    c = R.Cache(rng, [x + d for x, d in zip(ctx, nd)], kv=kv, hd=hd, f32=t == "f32", width=1 << 12).up()
+    q = rng.standard_normal((n, T, heads * hd)).astype(np.float32) * 2
+    mask = R.words(np.stack([R.ancestors(rng, T) for _ in range(n)]))
+    slots = rng.permutation(n)
+    slots[-1] = n + 3
+    pick = lambda a: [a[i] if i < n else 5 for i in slots]  # noqa: E731
+    got = run_tree(c, 0, q, pick(ctx), pick(nd), mask, heads, slots)
+    want = R.tree_rows(c, 0, q, pick(ctx), pick(nd), mask, heads, np.full(q.shape, 7.5), slots)
+    for i in range(n - 1):
+        assert (got[i, pick(nd)[i]:] == 7.5).all()
+    assert (got[-1] == 7.5).all()
+    close(got, want, R.attn_tol(hd, 4100, q, c.k), c.v[np.isfinite(c.v)])
+    again = run_tree(c, 0, q, pick(ctx), pick(nd), mask, heads, slots)
+    assert np.array_equal(got, again)
+
+
+def test_nothing_to_do_in_a_long_table():
+    rng = np.random.default_rng(26)
+    c = R.Cache(rng, [5, 0], kv=2, hd=64, width=1 << 14).up()
+    q = rng.standard_normal((2, 40, 8 * 64)).astype(np.float32)
+    assert (run_tree(c, 0, q, [5, 0], [0, 0], None, 8) == 7.5).all()
+
+
+def test_drafts_longer_than_a_step():
+    """300 tokens: masks of ten words, windows that begin inside a word; and a chain of them."""
+    rng = np.random.default_rng(27)
+    T = 300
+    c = R.Cache(rng, [77 + T], kv=1, hd=64).up()
+    q = rng.standard_normal((1, T, 64)).astype(np.float32) * 2
+    for mask in (R.words(R.ancestors(rng, T)[None]), None):
+        got = run_tree(c, 0, q, [77], [T], mask, 1)
+        close(got, R.tree_rows(c, 0, q, [77], [T], mask, 1, np.zeros(q.shape)), R.attn_tol(64, 77 + T, q, c.k), c.v)
+
+
+def test_compact_of_long_paths():
+    """More rows than a block finds at once, over page borders, every place a source of a later one."""
+    rng = np.random.default_rng(28)
+    T = 260
+    c = R.Cache(rng, [30 + T, 5 + T], kv=2, hd=64, layers=2).up()
+    path = np.stack([np.sort(rng.choice(T, 200, replace=False)) for _ in range(2)]).astype(u32)
+    path[0, 150:] = path[0, 149]  # ends here
+    start = [30, 5]
+    K.pages_compact(c.pages, c.seqs, dev([0, 1], u32), dev(start, u32), dev(path), dev([200, 193], u32), 2, 200)
+    for s, n in ((0, 150), (1, 193)):
+        for j in range(n):
+            a, b = start[s] + int(path[s, j]), start[s] + j
+            for pool in (c.k, c.v):
+                pool[:, c.table[s, b // 16], :, b % 16] = pool[:, c.table[s, a // 16], :, a % 16]
+    assert np.array_equal(c.dk.numpy(), c.k, equal_nan=True) and np.array_equal(c.dv.numpy(), c.v, equal_nan=True)
+
+
+def test_sparse_over_thousands_of_pages():
+    rng = np.random.default_rng(29)
+    c = R.Cache(rng, [16 * 2600 - 3, 100], kv=1, hd=64).up()
+    q = rng.standard_normal((2, 2 * 64)).astype(np.float32)
+    b = all_bounds(c, 0)
+    b[c.table[0, 1000], 0, 1, 5] = np.inf
+    ctx = [int(x) for x in c.len]
+    for take in (1, 40, 2599):
+        got, taken = run_sparse(c, 0, q, ctx, b, 2, take, 0, min(1, take - 1))
+        for s in range(2):
+            assert np.array_equal(taken[s], R.choose(c, s, q[s], ctx[s], b, 2, take, 0, min(1, take - 1))), (take, s)
+        assert 1000 in taken[0]
+        close(got[0], R.sparse_rows(c, 0, 0, q[0], ctx[0], taken[0], 2), R.attn_tol(64, take * 16, q, c.k), c.v)
 
 
 # ------------------------------------------------------------------- pages

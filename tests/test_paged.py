@@ -142,6 +142,12 @@ def test_attention_shapes():
         refused(lambda: K.tree_attn_workspace(p, t, 1, 4, heads), "query heads", -2)
         refused(lambda: K.sparse_attn(p, t, 0, B, B, B, 1, heads, 4, 1, 1, B, B, 1 << 40, B), "query heads", -2)
     refused(lambda: K.tree_attn(p, t, 0, B, B, B, B, 1, 1025, 6, B, 1 << 40, B), "at most 1024", -2)
+    one = pages(n_kv_heads=1)
+    refused(lambda: K.tree_attn(one, t, 0, B, B, B, B, 1, 1024, 65, B, 1 << 40, B), "at most 65536 rows", -2)
+    assert K.tree_attn_workspace(one, t, 1, 1024, 64) >= 0
+    many = pages(n_kv_heads=1024, n_pages=4)
+    refused(lambda: K.tree_attn_workspace(many, t, 0xFFFF, 1, 1024), "too many for one call")
+    refused(lambda: K.tree_attn_workspace(one, table(max_pages=(1 << 27) - 1), 1024, 1024, 8), "too many for one call")
     refused(lambda: K.tree_attn(p, t, 0, B, B, B, B, 1 << 16, 1, 6, B, 1 << 40, B), "at most 65535")
     refused(lambda: K.page_bounds(p, t, 0, B, B, 1 << 16, B), "at most 65535")
     refused(lambda: K.tree_attn(p, t, 0, Ptr(0x10004), B, B, B, 1, 4, 6, B, 1 << 40, B), "16-byte")
