@@ -84,9 +84,16 @@ __device__ __forceinline__ Seq seq_of(const LkPagedAttn& a, uint32_t s) {
     }
     return q;
 }
-__device__ __forceinline__ uint32_t chunks_of(uint32_t total, uint32_t chunk) {
-    const uint32_t c = (total + chunk - 1) / chunk;
-    return c ? c : 1;
+// A sequence's chunks: as many as the table's capacity has (a short one is spread as wide), each of a.chunk
+// positions at least, in whole steps of the workgroup.  (Chunks of the capacity's size: 17.0 us for one token over 4000
+// positions where the table has room for 65536, here 10.3.)
+struct Chunks {
+    uint32_t size, count;
+};
+__device__ __forceinline__ Chunks chunks_of(const LkPagedAttn& a, uint32_t total) {
+    const uint32_t units = (total + (1u << a.unit) - 1) >> a.unit, even = (units + a.n_chunks - 1) / a.n_chunks << a.unit;
+    const uint32_t size = even > a.chunk ? even : a.chunk, count = (total + size - 1) / size;
+    return Chunks{size, count ? count : 1};
 }
 
 // A workgroup's share: some of the positions of a (sequence, kv head), and one group of its rows.
@@ -112,11 +119,12 @@ __device__ __forceinline__ Share share_of(const LkPagedAttn& a, uint32_t rows) {
     h.sq = seq_of<SPARSE>(a, h.s);
     h.R = h.sq.rows * a.G;
     h.row0 = rg * rows;
-    h.x0 = chunk * a.chunk;
-    h.live = h.sq.live && h.row0 < h.R && (h.x0 < h.sq.total || chunk == 0);
-    h.whole = chunks_of(h.sq.total, a.chunk) == 1;
+    const Chunks of = chunks_of(a, h.sq.total);
+    h.x0 = chunk * of.size;
+    h.live = h.sq.live && h.row0 < h.R && chunk < of.count;
+    h.whole = of.count == 1;
     h.part = ((size_t)pair * a.n_chunks + chunk) * a.rows_pad + h.row0;
-    h.x1 = h.x0 + a.chunk < h.sq.total ? h.x0 + a.chunk : h.sq.total;
+    h.x1 = h.x0 + of.size < h.sq.total ? h.x0 + of.size : h.sq.total;
     return h;
 }
 
@@ -1069,7 +1077,7 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const LkPagedAttn a) {
         base = wg * 2 * RG + row % RG;
         stride = 2 * RG;
     } else {
-        parts = chunks_of(sq.total, a.chunk);
+        parts = chunks_of(a, sq.total).count;
         base = (size_t)pair * a.n_chunks * a.rows_pad + row;
         stride = a.rows_pad;
     }
@@ -1142,6 +1150,8 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
         if (!p.chunk) p.chunk = all;
         p.n_chunks = (uint32_t)((positions + p.chunk - 1) / p.chunk);
         if (!p.n_chunks) p.n_chunks = 1;
+        while (1u << p.unit < all) p.unit++;  // a power of two
+        if (p.narrow) p.chunk = p.n_chunks > 1 ? all : p.chunk;
         const uint64_t items = (uint64_t)n * n_kv * p.n_chunks;
         p.blocks = (items + 7) / 8 * 8 * p.n_rg;
         p.part_rows = p.n_chunks > 1 ? items * p.rows_pad : 0;
@@ -1181,6 +1191,7 @@ static hipError_t launch(const LkPagedAttn& a, const LkPagedPlan& p, hipStream_t
 
 hipError_t lk_paged_attn_launch(LkPagedAttn a, const LkPagedPlan& p, void* ws, hipStream_t st) {
     a.chunk = p.chunk;
+    a.unit = p.unit;
     a.n_chunks = p.n_chunks;
     a.n_rg = p.n_rg;
     a.rows_pad = p.rows_pad;

@@ -62,14 +62,14 @@ struct LkPagedAttn {
     // set by the launch
     float *part_ml, *part_o;
     uint64_t* place;       // wide: steps of a run, then where each sequence's steps begin
-    uint32_t chunk;        // positions of a chunk
+    uint32_t chunk, unit;  // positions of a chunk: at least, and log2 of what they are a multiple of
     uint32_t n_chunks, n_rg, rows_pad;
     float scale;           // log2(e) / sqrt(hd)
 };
 struct LkPagedPlan {
     bool narrow;           // waves take positions in turn; else they lie side by side in rows
     uint32_t tiles, waves; // 16-row tiles of a wave, waves of a workgroup
-    uint32_t chunk, n_chunks, n_rg, rows_pad;
+    uint32_t chunk, unit, n_chunks, n_rg, rows_pad;
     uint64_t blocks, steps;  // steps: of all items at the table's capacity
     uint64_t place_bytes, part_rows, part_bytes;
 };
