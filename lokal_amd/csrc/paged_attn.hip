@@ -41,7 +41,8 @@
 namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __fp16 p2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
+typedef float fl2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -341,14 +342,14 @@ struct Rows {
         for (int rt = 0; rt < RT; rt++) {
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {  // truncated to f16; what that leaves fits f16's 11 bits but for two
-                const float p0 = __builtin_amdgcn_exp2f(sc[rt][2 * g + e / 2][2 * (e & 1)]),
-                            p1 = __builtin_amdgcn_exp2f(sc[rt][2 * g + e / 2][2 * (e & 1) + 1]);
-                l[rt] += p0 + p1;
-                const p2 u = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+            for (int e = 0; e < 4; e++) {
+                const fl2 p = fl2{__builtin_amdgcn_exp2f(sc[rt][2 * g + e / 2][2 * (e & 1)]),
+                                  __builtin_amdgcn_exp2f(sc[rt][2 * g + e / 2][2 * (e & 1) + 1])};
+                l[rt] += p[0] + p[1];
+                const hf2 u = __builtin_convertvector(p, hf2);
                 hi[e] = __builtin_bit_cast(uint32_t, u);
-                lo[e] = __builtin_bit_cast(
-                    uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)u[0], minus, p0), __builtin_fmaf((float)u[1], minus, p1)));
+                const fl2 rest = fl2{__builtin_fmaf((float)u[0], minus, p[0]), __builtin_fmaf((float)u[1], minus, p[1])};
+                lo[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, hf2));
             }
             ph[rt] = __builtin_bit_cast(h8, u4{hi[0], hi[1], hi[2], hi[3]});
             pl[rt] = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
@@ -648,7 +649,6 @@ __device__ __forceinline__ uint32_t row_groups(const LkPagedAttn& a, const Seq& 
     return q.live ? (q.rows * a.G + rows - 1) / rows : 0;
 }
 constexpr uint32_t kLeast = 2;  // steps of a run at least
-constexpr uint32_t kOcc = 2;    // waves of the wide kernel on a SIMD: 256 registers each
 
 // All workgroups count all sequences; `start`: where this one's run begins.  Sequences are read twice (total, then
 // the place) unless one round of the threads holds them.  Workgroup 0 leaves the sequences' places for the fold.
@@ -741,9 +741,11 @@ struct Wide {
     static constexpr int NT = F32 || HD == 128 ? 2 : 4, STEP = NT * 16, ROWS = NW * 32;
     static constexpr int SIDE = STEP * HD * (F32 ? 4 : 2);  // bytes of a step's K or V
     static constexpr int RING = F32 ? 1 : SIDE <= 8192 && NW == 4 ? 3 : 2;
+    // Waves on a SIMD: two of 256 registers, but where two waves share 64 KB of LDS two such workgroups fill a CU.
+    static constexpr int OCC = F32 && HD == 128 && NW == 2 ? 1 : 2;
 };
 template <int HD, bool F32, int NW>
-__global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPagedAttn a) {
+__global__ __launch_bounds__(NW * 64, (Wide<HD, F32, NW>::OCC)) void paged_wide_kernel(const LkPagedAttn a) {
     constexpr int RT = 2, NT = Wide<HD, F32, NW>::NT, STEP = Wide<HD, F32, NW>::STEP, ROWS = Wide<HD, F32, NW>::ROWS;
     using Wave = Rows<HD, false, RT, NT, false, true>;
     constexpr int ND = Wave::ND, KS = Wave::KS, ES = F32 ? 4 : 2;
@@ -900,24 +902,39 @@ __global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPaged
                 for (int side = 0; side < 2; side++)
 #pragma unroll
                     for (uint32_t e = 0; e < EACH; e++) {
-                        const uint32_t at = threadIdx.x + e * NW * 64, row = at / (HD / 8);
-                        const f4* from = (const f4*)(ring[0] + side * SIDE + at * 32);
-                        const bool see = !side || !masked || live >> row & 1;
+                        const f4* from = (const f4*)(ring[0] + side * SIDE + (threadIdx.x + e * NW * 64) * 32);
+                        u[side][e][0] = from[0], u[side][e][1] = from[1];
+                    }
+                if (masked) {
 #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            f4 y = from[k];
+                    for (uint32_t e = 0; e < EACH; e++) {
+                        const bool see = live >> ((threadIdx.x + e * NW * 64) / (HD / 8)) & 1;
 #pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const bool bad = not_finite(y[i]);
-                                if (side && masked) {
-                                    any |= see && bad;
-                                    y[i] = see && !bad ? y[i] : 0.f;
-                                }
-                                top[side] = fmaxf(top[side], bad ? 0.f : fabsf(y[i]));
-                            }
-                            u[side][e][k] = y;
+                        for (int i = 0; i < 8; i++) {
+                            const float y = u[1][e][i / 4][i % 4];
+                            const bool bad = not_finite(y);
+                            any |= see && bad;
+                            u[1][e][i / 4][i % 4] = see && !bad ? y : 0.f;
                         }
                     }
+                }
+#pragma unroll
+                for (int side = 0; side < 2; side++) {
+#pragma unroll
+                    for (uint32_t e = 0; e < EACH; e++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) top[side] = fmaxf(top[side], fabsf(u[side][e][i / 4][i % 4]));
+                    if (__any(top[side] == INFINITY)) {  // the largest finite one
+                        top[side] = 0.f;
+#pragma unroll
+                        for (uint32_t e = 0; e < EACH; e++)
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                const float y = u[side][e][i / 4][i % 4];
+                                top[side] = fmaxf(top[side], not_finite(y) ? 0.f : fabsf(y));
+                            }
+                    }
+                }
 #pragma unroll
                 for (int side = 0; side < 2; side++) {
                     const float t = lk_wave_max(top[side]);
@@ -950,6 +967,9 @@ __global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPaged
                     v_up = up[1];
                 }
                 up[1] = v_up;
+                float minus = -1.f;  // as in weights()
+                asm("" : "+s"(minus));
+                const float by[2] = {ldexpf(1.f, up[0]), ldexpf(1.f, up[1])};  // -115..126: a normal number
 #pragma unroll
                 for (int side = 0; side < 2; side++)
 #pragma unroll
@@ -957,10 +977,13 @@ __global__ __launch_bounds__(NW * 64, kOcc) void paged_wide_kernel(const LkPaged
                         const uint32_t at = threadIdx.x + e * NW * 64, row = at / (HD / 8), piece = (at % (HD / 8)) ^ (row & 7);
                         h8 hi, lo;
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float y = ldexpf(u[side][e][i / 4][i % 4], up[side]);
-                            hi[i] = (_Float16)y;
-                            lo[i] = (_Float16)(y - (float)hi[i]);
+                        for (int i = 0; i < 8; i += 2) {
+                            const fl2 y = fl2{u[side][e][i / 4][i % 4] * by[side], u[side][e][i / 4][i % 4 + 1] * by[side]};
+                            const hf2 x = __builtin_convertvector(y, hf2);
+                            const hf2 z = __builtin_convertvector(
+                                (fl2{__builtin_fmaf((float)x[0], minus, y[0]), __builtin_fmaf((float)x[1], minus, y[1])}), hf2);
+                            hi[i] = x[0], hi[i + 1] = x[1];
+                            lo[i] = z[0], lo[i + 1] = z[1];
                         }
                         char* to = s_parts + side * 2 * PART + row * ROW + piece * 16;
                         *(h8*)to = hi;
@@ -1122,7 +1145,7 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
     p.rows_pad = p.n_rg * per;
     const uint64_t base = (uint64_t)n * n_kv * p.n_rg;
     const uint32_t step = f32 || hd == 128 ? 32 : 64;
-    const uint64_t steps = (positions + step - 1) / step, fill = (uint64_t)kCus * kOcc * 4 / p.waves;
+    const uint64_t steps = (positions + step - 1) / step, fill = (uint64_t)kCus * (p.waves == 4 || (f32 && hd == 128) ? 2 : 4);
     p.steps = base * steps;
     // Runs begin 7 us later than chunks (they count the work first) and pay from about 480 positions a workgroup on, 240
     // of an f32 cache.  us, chunks / runs: 4 x 32 tokens, 32 / 4 heads of 64, up to 4096 positions (256 a workgroup) 25 /
