@@ -1147,11 +1147,12 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
     const uint32_t step = f32 || hd == 128 ? 32 : 64;
     const uint64_t steps = (positions + step - 1) / step, fill = (uint64_t)kCus * (p.waves == 4 || (f32 && hd == 128) ? 2 : 4);
     p.steps = base * steps;
-    // Runs begin 7 us later than chunks (they count the work first) and pay from about 480 positions a workgroup on, 240
-    // of an f32 cache.  us, chunks / runs: 4 x 32 tokens, 32 / 4 heads of 64, up to 4096 positions (256 a workgroup) 25 /
-    // 30, 8192 (512) 44 / 35; 24 x 12, 32 / 8 of 128, 2048 (390) 51 / 59, 8 x 16, 8192 (512) 80 / 74; f32, 3 x 23, 32 / 8
-    // of 128, 5000 (236) 59 / 64, 4 x 16, 8192 (256) 169 / 100.
-    if (!p.narrow && p.steps * step > (f32 ? 240 : 480) * fill) {
+    // Runs begin 7 us later than chunks (they count the work first), but share out what lengths there are; chunks are as
+    // long as the longest sequence's.  Runs from 480 positions a workgroup on.  us, chunks / runs: sequences of one
+    // length, 8 x 16 tokens, 32 / 8 heads of 128, 8192 positions (512 a workgroup) 86 / 90; 4 x 32, 32 / 4 of 64, 8000 of
+    // 8192 (512) 69 / 74, 1000 of 4096 (256) 33 / 34; f32, 3 x 23, 32 / 8 of 128, 5000 (236) 56 / 64; of many lengths,
+    // 8 x 64, up to 32768 (4096) 251 / 171.
+    if (!p.narrow && p.steps * step > 480 * fill) {
         p.blocks = fill;
         p.part_rows = fill * 2 * per;
         p.place_bytes = (((uint64_t)n + 1) * 8 + 255) / 256 * 256;
@@ -1162,9 +1163,13 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
         if (p.narrow) {
             // two steps a wave cost less than a fold: 1 x 1 token, up to 304 positions, 9.4 -> 8.6 us
             c = pieces <= 2 ? 1 : (1024 + base - 1) / base;
-        } else {  // chunks of 512 positions, shorter ones if that leaves too few
-            const uint64_t by_len = (positions + 511) / 512, by_fill = (512 + base - 1) / base;
-            c = by_len > by_fill ? by_len : by_fill;
+        } else {  // as few rounds of the card as can be, each of a chunk's positions and some 128 to begin
+            uint64_t least = ~0ull;
+            c = 1;
+            for (uint64_t k = 1; k <= kMaxChunks && k <= pieces; k++) {
+                const uint64_t cost = (base * k + fill - 1) / fill * ((pieces + k - 1) / k * all + 128);
+                if (cost < least) least = cost, c = k;
+            }
         }
         c = c > kMaxChunks ? kMaxChunks : c;
         c = c > pieces ? pieces : c;
@@ -1174,7 +1179,9 @@ LkPagedPlan lk_paged_plan(uint32_t hd, bool f32, bool sparse, uint32_t n, uint32
         p.n_chunks = (uint32_t)((positions + p.chunk - 1) / p.chunk);
         if (!p.n_chunks) p.n_chunks = 1;
         while (1u << p.unit < all) p.unit++;  // a power of two
-        if (p.narrow) p.chunk = p.n_chunks > 1 ? all : p.chunk;
+        // short sequences: chunks down to this.  f32, 3 x 23 tokens over 1000 positions, 5000 in the table: 37 -> 29 us
+        const uint32_t spread = p.narrow ? all : f32 ? 128 : 256;
+        if (p.n_chunks > 1 && p.chunk > spread) p.chunk = spread;
         const uint64_t items = (uint64_t)n * n_kv * p.n_chunks;
         p.blocks = (items + 7) / 8 * 8 * p.n_rg;
         p.part_rows = p.n_chunks > 1 ? items * p.rows_pad : 0;
