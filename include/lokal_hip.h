@@ -427,8 +427,8 @@ int lkhip_pages_compact(const lkhip_kv_pages* pages, const lkhip_page_table* tab
  * zeros; rows at and behind n_draft[i] are left as they were.  n_draft NULL: all
  * have max_draft.  max_draft <= 1024; n_heads a multiple of the kv heads, at most
  * 65536 / max_draft for each of them.  Positions that a row does not see do
- * not reach it, whatever they hold; one that it sees with a K or V that is not
- * finite makes it not finite.  Needs lkhip_tree_attn_workspace bytes (16-byte
+ * not reach it, whatever they hold; one that it sees with a V that is not finite
+ * makes it not finite, one with such a K can.  q and out must not overlap.  Needs lkhip_tree_attn_workspace bytes (16-byte
  * aligned, any content), in use until the call's work is done: two calls that
  * can run at once need two. */
 int lkhip_tree_attn_workspace(const lkhip_kv_pages* pages, const lkhip_page_table* table, size_t n, size_t max_draft,

@@ -208,6 +208,11 @@ static int plan_of(const LkPages& p, const LkTable& t, size_t n, size_t tokens, 
                     who, n, tokens, n_heads, (unsigned long long)cap);
     return LKHIP_OK;
 }
+static int apart(const float* q, const float* out, size_t count, const char* who) {
+    if ((uintptr_t)q < (uintptr_t)(out + count) && (uintptr_t)out < (uintptr_t)(q + count))
+        return fail(LKHIP_E_INVALID, "%s: q and out overlap", who);
+    return LKHIP_OK;
+}
 static int ws_check(const void* ws, size_t have, size_t need, const char* who) {
     if (need && (!ws || have < need || !aligned(ws, 16)))
         return fail(LKHIP_E_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", who, need,
@@ -246,6 +251,7 @@ extern "C" int lkhip_tree_attn(const lkhip_kv_pages* pages, const lkhip_page_tab
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(LKHIP_E_INVALID, "%s: q and out must be 16-byte aligned", who);
     CHECK(plan_of(p, t, n, max_draft, n_heads, 0, who, plan, keys, bytes));
     CHECK(ws_check(ws, ws_bytes, bytes, who));
+    CHECK(apart(q, out, n * max_draft * n_heads * p.hd, who));
     LkPagedAttn a{};
     a.p = p;
     a.t = t;
@@ -302,6 +308,7 @@ extern "C" int lkhip_sparse_attn(const lkhip_kv_pages* pages, const lkhip_page_t
         return fail(LKHIP_E_INVALID, "%s: q, bounds and out must be 16-byte aligned", who);
     CHECK(plan_of(p, t, n, 1, n_heads, n_take, who, plan, keys, bytes));
     CHECK(ws_check(ws, ws_bytes, bytes, who));
+    CHECK(apart(q, out, n * n_heads * p.hd, who));
     LkSparse c{};
     c.p = p;
     c.t = t;

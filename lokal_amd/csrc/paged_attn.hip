@@ -16,16 +16,17 @@
 //     index is taken as those positions; V is read with the same positions and
 //     neighbouring dims per lane, so O's lanes hold neighbouring dims.
 // q carries log2(e) / sqrt(hd).  f16 cache: K and V are exact operands; q (scaled
-// per row by a power of two, so that its largest value is in 2^13..2^14) and P are
-// each split into two f16 parts (22 bits), as one part alone is off by 1.4e-4.
-// f32 cache: 16x16x4 f32 products.
+// per row by a power of two where its values need it) and P are each split into two
+// f16 parts (22 bits), as one part alone is off by 1.4e-4.  f32 cache: 16x16x4 f32
+// products up to 32 rows; more rows split K and V into two f16 parts too and take
+// three of the four products (76 -> 64 us for 3 x 23 tokens when it came).
 // The running maximum lags: it moves when some score passes it by 8 (in log2),
 // so most steps neither reduce over lanes nor rescale O; P stays below 2^8.
 //
 // Two kernels.  Up to 32 rows (narrow): the four waves of a workgroup take steps in
-// turn, K and V go straight from memory to registers, and the waves join at the end.  More rows (wide): the waves lie
-// side by side in rows and share each step's K and V through LDS, a ring of stages
-// that loads write without registers.
+// turn, K and V go straight from memory to registers, and the waves join at the end.
+// More rows (wide): the waves lie side by side in rows and share each step's K and V
+// through LDS, a ring of stages that loads write without registers.
 //
 // Positions that no row sees (behind the draft, in holes of the table) are clamped
 // to readable rows; their scores become -inf and their V zero, so what lies there
@@ -482,6 +483,10 @@ struct Rows {
 
 // ---------------------------------------------------------------- narrow
 
+// Bound by memory where there is work for the card: 32 sequences x 8 kv heads x 1536 positions of 128 (201 MB) 46.9 us,
+// 4.3 TB/s; below that by a chain of dependent reads (length, page id, K) and the join: 1 x 1 token over 304 positions
+// 8.7 us, 4 x 2 kv heads x 4096 positions 8.1 us.  All loads of a step go out before the first product; three waves a
+// SIMD (head 64) hide them better than two with a step ahead.
 template <int HD, bool F32, int RT, bool SPARSE>
 __global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow_kernel(const LkPagedAttn a) {
     constexpr int NT = F32 || HD == 128 ? 2 : 4, W = 4, ROWS = RT * 16, STEP = NT * 16;
@@ -638,8 +643,8 @@ __global__ __launch_bounds__(256, RT == 1 && HD == 64 ? 3 : 2) void paged_narrow
 // Work of the wide kernel is counted in steps of an item: a (sequence, kv head, group of ROWS rows), all items one
 // after the other, row groups of a kv head together.  How many there are is known on the device only (contexts and
 // drafts differ), so a fixed number of workgroups, as many as the card holds at once, takes equal runs of steps; a run
-// may end one item and begin others.  Fixed chunks of the table's capacity left half the card idle behind the last
-// of 565 live workgroups on 512 places (8 x 64 tokens over up to 32768 positions: 214 us).
+// may end one item and begin others.  Chunks, as long as the longest sequence's, leave the card idle
+// behind the shorter ones: 8 x 64 tokens over up to 32768 positions 251 us against 171.
 struct Plan {
     uint32_t total, run;  // steps in all (the host keeps them below 2^32) and of a workgroup
 };
@@ -736,6 +741,12 @@ __device__ __forceinline__ Plan plan_runs(const LkPagedAttn& a, uint32_t wg, uin
 // ahead; one barrier a step.  A place there holds rows of RB bytes, whose 16-byte pieces lie at their number ^ (row &
 // 7), so that eight lanes that read one piece of eight rows meet eight different bank groups.  Loads write LDS in lane
 // order, so the lane that lands in a place fetches the piece that belongs there.
+// f32 cache: a step lands once, each thread takes its values to registers, the next step's loads go out, and the two f16
+// parts are written to a place of their own: three barriers a step.
+// What bounds it.  Many rows: the matrix cores and the adders in turn (31% and 41% of their cycles): 8 x 64 tokens, 32 / 4
+// heads of 64, all over 32768 positions 374 us, 736 TFLOP/s with both parts counted, 67% of a large library product's.
+// Few rows: the chain of a step's landing, products and weights in a workgroup: 24 x 12 tokens, 32 / 8 heads of 128, up
+// to 2048 positions 43.6 us for 132 MB; f32, 3 x 23 tokens, up to 5000 positions 44.5 us for 77 MB.
 template <int HD, bool F32, int NW>
 struct Wide {
     static constexpr int NT = F32 || HD == 128 ? 2 : 4, STEP = NT * 16, ROWS = NW * 32;
@@ -1077,8 +1088,8 @@ __global__ __launch_bounds__(NW * 64, (Wide<HD, F32, NW>::OCC)) void paged_wide_
 
 // Parts of a row, joined.  A block takes four rows: a wave weighs a row's parts (lane = part, at most 64), then HD / 4
 // lanes by SPLIT groups a row add them up, each group every SPLIT-th part: two dependent reads of memory in all.  (One
-// thread group walking the parts of a row: 19.6 us for 33 parts of 112 rows x 8.)  ROWS: of a workgroup of the wide
-// kernel; 0: parts are the narrow kernel's chunks.
+// thread group walking the parts of a row: 19.6 us for 33 parts of 112 rows x 8; now 4.3 us.)  ROWS: of a workgroup of
+// the wide kernel; 0: parts are the narrow kernel's chunks.
 template <int HD, bool SPARSE, int ROWS, uint32_t STEP>
 __global__ __launch_bounds__(256) void paged_fold_kernel(const LkPagedAttn a) {
     constexpr uint32_t L = HD / 4, SPLIT = 64 / L;

@@ -311,6 +311,32 @@ def test_long_tables_over_runs_of_steps(t, hd, heads, kv, T, n):
     assert np.array_equal(got, again)
 
 
+@pytest.mark.parametrize("heads", [3, 20, 60])
+@pytest.mark.parametrize("t,hd", [("f16", 64), ("f16", 128), ("f32", 64), ("f32", 128)])
+def test_short_sequences_in_a_long_table(t, hd, heads):
+    """Chunks follow a sequence's own length: none, one position, about a chunk, the table's whole capacity."""
+    rng = np.random.default_rng(hd + heads)
+    T, ctx = 2, [0, 1, 126, 127, 128, 254, 255, 256, 600, 3000, 4094]
+    c = R.Cache(rng, [x + T for x in ctx], kv=1, hd=hd, f32=t == "f32", width=256).up()
+    q = rng.standard_normal((len(ctx), T, heads * hd)).astype(np.float32)
+    got = run_tree(c, 0, q, ctx, None, None, heads)
+    want = R.tree_rows(c, 0, q, ctx, [T] * len(ctx), None, heads, np.full(q.shape, 7.5))
+    close(got, want, R.attn_tol(hd, 4096, q, c.k), c.v)
+
+
+@pytest.mark.parametrize("t,hd,heads", [("f16", 128, 9), ("f16", 64, 17), ("f32", 64, 5), ("f32", 128, 8)])
+def test_sparse_of_many_heads_over_long_tables(t, hd, heads):
+    rng = np.random.default_rng(hd * heads)
+    ctx = [16 * 500 - 1, 16 * 300, 40]
+    c = R.Cache(rng, ctx, kv=1, hd=hd, f32=t == "f32").up()
+    q = rng.standard_normal((3, heads * hd)).astype(np.float32)
+    b = all_bounds(c, 0)
+    got, taken = run_sparse(c, 0, q, ctx, b, heads, 20, 1, 2)
+    for s in range(3):
+        assert np.array_equal(taken[s], R.choose(c, s, q[s], ctx[s], b, heads, 20, 1, 2)), s
+        close(got[s], R.sparse_rows(c, 0, s, q[s], ctx[s], taken[s], heads), R.attn_tol(hd, 320, q, c.k), c.v)
+
+
 def test_nothing_to_do_in_a_long_table():
     rng = np.random.default_rng(26)
     c = R.Cache(rng, [5, 0], kv=2, hd=64, width=1 << 14).up()

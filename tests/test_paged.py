@@ -174,3 +174,12 @@ def test_workspaces_do_not_grow_with_what_a_sequence_holds():
     a = K.tree_attn_workspace(pages(n_pages=64), t, 4, 16, 14)
     assert a == K.tree_attn_workspace(pages(n_pages=8192), t, 4, 16, 14)
     assert K.tree_attn_workspace(pages(), t, 0, 16, 14) == 0 == K.tree_attn_workspace(pages(), t, 4, 0, 14)
+
+
+def test_q_and_out_are_apart():
+    rows = 2 * 4 * 6 * 64 * 4  # bytes of q, and of out
+    for at in (0, 16, rows - 16, -16, 16 - rows):
+        out = Ptr(0x100000 + at)
+        refused(lambda: K.tree_attn(pages(), table(), 0, Ptr(0x100000), B, B, B, 2, 4, 6, B, 1 << 40, out), "overlap")
+        if abs(at) < rows // 4:
+            refused(lambda: K.sparse_attn(pages(), table(), 0, Ptr(0x100000), B, B, 2, 6, 4, 1, 1, B, B, 1 << 40, out), "overlap")
