@@ -96,7 +96,7 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* part, 
 // does not exist, came before, has no room, or where the free pages end
 // before its last one; entries that need none are never refused for that.
 // T: threads, at least n; kScan refs a thread looks at in one go.  Bound by its chain
-// of reads and barriers: 5.2 us for 2 entries over 64 pages, 9.9 for 48 over 4096.
+// of reads and barriers: 5.4 us for 2 entries and a page, 9.9 for 48 and two pages each.
 // One workgroup, as the order of the list decides who gets a page.
 template <uint32_t T>
 __global__ __launch_bounds__(T) void pages_grow_kernel(LkPages p, LkTable t, const uint32_t* slots,
