@@ -20,8 +20,9 @@
 // f16 parts (22 bits), as one part alone is off by 1.4e-4.  f32 cache: 16x16x4 f32
 // products up to 32 rows; more rows split K and V into two f16 parts too and take
 // three of the four products (76 -> 64 us for 3 x 23 tokens when it came).
-// The running maximum lags: it moves when some score passes it by 8 (in log2),
-// so most steps neither reduce over lanes nor rescale O; P stays below 2^8.
+// The running maximum lags: it moves when some score passes it by 6 (in log2),
+// so most steps neither reduce over lanes nor rescale O; f16 parts of P are
+// held 2^9 times and stay below 2^15, sums and O alike.
 //
 // Two kernels.  Up to 32 rows (narrow): the four waves of a workgroup take steps in
 // turn, K and V go straight from memory to registers, and the waves join at the end.
@@ -50,7 +51,10 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
 #define LK_INLINE __attribute__((always_inline))  // lambdas too: what they capture stays in registers
-constexpr float kLag = 8.f;  // log2: how far a score may pass the running maximum
+constexpr float kLag = 6.f;  // log2: how far a score may pass the running maximum
+// Weights are held 2^kUp times: with kLag below 2^15, and small ones keep bits in f16, whose steps end at 2^-24.  (At
+// once their size, 4096 weights of 2^-17 beside one of 1 were off by 2^-25 each, all to one side: 1.2e-4 of the sum.)
+constexpr float kUp = 9.f;
 constexpr uint32_t kMaxChunks = 64;
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
@@ -160,6 +164,7 @@ template <int HD, bool F32, int RT, int NT, bool SPARSE, bool TR>
 struct Rows {
     static constexpr int ND = HD / 16, KS = F32 ? ND : HD / 32, ES = F32 ? 4 : 2;
     static constexpr int VW = ND * ES / 4;  // words of a lane's dims of one V row
+    static constexpr float UP = F32 ? 0.f : kUp;  // weights in f32 need none
     h8 qh[F32 ? 1 : RT][F32 ? 1 : KS], ql[F32 ? 1 : RT][F32 ? 1 : KS];
     f4 qf[F32 ? RT : 1][F32 ? ND : 1];
     float m[RT];     // log2: what row c16's weights are relative to; -inf before its first score
@@ -288,12 +293,12 @@ struct Rows {
             for (int i = 0; i < 4; i++) sc[rt][t][i] = b[t / 2] >> (16 * (t & 1) + i) & 1 ? sc[rt][t][i] : -INFINITY;
     }
 
-    // Products of K times 2^k_up become scores relative to m.
+    // Products of K times 2^k_up become scores relative to m, and UP.
     __device__ __forceinline__ void relate(Scores& sc, int k_up) const {
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const int by = -(up[rt] + k_up);  // scores of 2^126 and more are all alike
-            const float f = ldexpf(1.f, by < 126 ? by : 126), z = m[rt] == -INFINITY ? 0.f : -m[rt];
+            const float f = ldexpf(1.f, by < 126 ? by : 126), z = m[rt] == -INFINITY ? 0.f : UP - m[rt];
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -311,7 +316,7 @@ struct Rows {
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) top[rt] = fmaxf(top[rt], sc[rt][t][i]);
-            far |= top[rt] > (m[rt] == -INFINITY ? -INFINITY : kLag);
+            far |= top[rt] > (m[rt] == -INFINITY ? -INFINITY : kLag + UP);
         }
         if (!__any(far)) return;
 #pragma unroll
@@ -320,7 +325,7 @@ struct Rows {
             float x = top[rt];
             x = fmaxf(x, __shfl_xor(x, 16, 64));
             x = fmaxf(x, __shfl_xor(x, 32, 64));
-            const float by = first ? (x == -INFINITY ? 0.f : x) : fmaxf(x, 0.f);  // how far m goes up
+            const float by = first ? (x == -INFINITY ? 0.f : x - UP) : fmaxf(x - UP, 0.f);  // how far m goes up; first: scores down
             const float f = first ? 1.f : __builtin_amdgcn_exp2f(-by);
             m[rt] = first ? x : m[rt] + by;
 #pragma unroll

@@ -324,6 +324,31 @@ def test_short_sequences_in_a_long_table(t, hd, heads):
     close(got, want, R.attn_tol(hd, 4096, q, c.k), c.v)
 
 
+@pytest.mark.parametrize("t", ["f16", "f32"])
+@pytest.mark.parametrize("heads", [1, 40])
+def test_many_small_weights_beside_a_large_one(t, heads):
+    """One position of weight 1 and V 0, the others of 2^-17 (1 + 2^-8) and V 1: many weights that all round alike.
+
+    So many sequences (of the same pages) that a wave's share is long, 4096 positions (heads 1).  A rounding of a sum
+    for each product of 32 positions and part, 2^-24 each, were one wave to take all.  The large score is off by 4 + 1
+    steps of its 17, times ln 2 on a weight; the small scores are exact, their weights off by 4 steps; 64 for the rest."""
+    n, length = 1024 if heads == 1 else 64, 16384
+    rng = np.random.default_rng(3)
+    c = R.Cache(rng, [length], kv=1, hd=64, page=256, f32=t == "f32")
+    c.k[...] = 0
+    c.v[...] = 1
+    c.k[0, c.table[0, 1], 0, 2, 0] = 1
+    c.v[0, c.table[0, 1], 0, 2] = 0
+    c.up()
+    low = 17 - np.log2(1 + 2.0 ** -8)
+    q = np.zeros((n, 1, heads * 64), np.float32)
+    q[:, :, ::64] = low * 8 / np.log2(np.e)
+    got = run_tree(c, 0, q, [length - 1] * n, None, None, heads, np.zeros(n, np.uint32))
+    w = (length - 1) * np.exp(-q[0, 0, 0].astype(np.float64) / 8)
+    tol = 2.0 ** -24 * (2 * length // 32 + 17 * 5 + 4 + 64)
+    assert np.abs(got - w / (1 + w)).max() <= tol * w / (1 + w)
+
+
 @pytest.mark.parametrize("t,hd,heads", [("f16", 128, 9), ("f16", 64, 17), ("f32", 64, 5), ("f32", 128, 8)])
 def test_sparse_of_many_heads_over_long_tables(t, hd, heads):
     rng = np.random.default_rng(hd * heads)
