@@ -405,15 +405,17 @@ int lkhip_pages_trim(const lkhip_kv_pages* pages, const lkhip_page_table* table,
 /* Row r of k and v (n_kv_heads * head_dim f32, ld floats apart, ld % 4 == 0,
  * 16-byte aligned) becomes position pos[r] of sequence slots[r] in one layer,
  * rounded to the cache's type (to nearest, as lokal's GPU cache,
- * src/gpu/metal.rs:3234-3235).  Rows of a call must have different places. */
+ * src/gpu/metal.rs:3234-3235).  Rows of a call must have different places.  They
+ * go where the table says, into a page that other sequences hold too as well:
+ * lkhip_pages_grow is what gives a sequence a last page of its own. */
 int lkhip_pages_write(const lkhip_kv_pages* pages, const lkhip_page_table* table, uint32_t layer, const float* k,
                       const float* v, size_t ld, const uint32_t* slots, const uint32_t* pos, size_t n_rows,
                       void* stream);
 /* The rows at positions from[i] + path[i][j] of sequence slots[i] move to
  * from[i] + j, j < n_path[i], in all layers: the accepted tokens of a draft
  * close up behind their context.  path: [n][ld_path], strictly increasing (it
- * ends at an entry that is not).  Rows in holes are left.  A slot named twice
- * is taken at its first place.  n <= 1024. */
+ * ends at an entry that is not).  Rows in holes are left; pages are written as by
+ * lkhip_pages_write.  A slot named twice is taken at its first place.  n <= 1024. */
 int lkhip_pages_compact(const lkhip_kv_pages* pages, const lkhip_page_table* table, const uint32_t* slots,
                         const uint32_t* from, const uint32_t* path, size_t ld_path, const uint32_t* n_path, size_t n,
                         void* stream);
